@@ -45,24 +45,6 @@ __global__ __launch_bounds__(64) void kern(float *out, float seed, unsigned long
       if (KIND == 28) asm volatile("v_fma_f32 %0, %0, %1, 1.0" : "+v"(a[i]) : "v"(m));
       if (KIND == 29) asm volatile("v_mul_f32 %0, 0.5, %0" : "+v"(a[i]));
     }
-    if (KIND == 30) {
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        float2 v = make_float2(a[i], a[i + 1]);
-        float2 mm = make_float2(m, m);
-        asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(v) : "v"(mm));
-        a[i] = v.x; a[i + 1] = v.y;
-      }
-    }
-    if (KIND == 4) {  // packed: 8 instructions on register pairs = 16 lane-fmas
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        float2 v = make_float2(a[i], a[i + 1]);
-        float2 mm = make_float2(m, m), cc = make_float2(c, c);
-        asm volatile("v_pk_fma_f32 %0, %0, %1, %2" : "+v"(v) : "v"(mm), "v"(cc));
-        a[i] = v.x; a[i + 1] = v.y;
-      }
-    }
   }
   const long long t1 = __builtin_amdgcn_s_memtime(), w1 = wall_clock64();
   if (blockIdx.x == 0 && threadIdx.x == 0) { out[512] = (float)(t1 - t0); out[513] = (float)(w1 - w0); }
@@ -92,13 +74,12 @@ void run(const char *name, float *d, int ninst) {
 int main() {
   float *d; hipMalloc(&d, 8192);
   run<0>("v_fma", d, 16); run<1>("v_mul", d, 16); run<2>("v_rcp", d, 16); run<3>("v_log", d, 16);
-  run<4>("v_pk_fma", d, 8); run<5>("v_med3", d, 16); run<6>("v_cndmask", d, 16);
+  run<5>("v_med3", d, 16); run<6>("v_cndmask", d, 16);
   run<7>("cndmask64", d, 16); run<8>("v_max", d, 16); run<9>("v_add", d, 16); run<10>("v_ldexp", d, 16);
   run<11>("mov_dpp", d, 16); run<12>("v_cmp", d, 16); run<13>("frexp_exp", d, 16); run<14>("v_exp", d, 16);
   run<15>("v_rsq", d, 16); run<16>("v_mul_b", d, 16); run<17>("v_fmac", d, 16);
   run<18>("cmp+cnd vcc (2)", d, 32); run<19>("cmp+cnd sgpr(2)", d, 32); run<20>("v_fmaak", d, 16); run<21>("v_mov", d, 16);
   run<22>("v_add_u32", d, 16); run<23>("fma neg", d, 16); run<24>("mul_e64 neg", d, 16); run<25>("v_min", d, 16);
   run<26>("v_lshlrev", d, 16); run<27>("v_cvt", d, 16); run<28>("fma inline1.0", d, 16); run<29>("mul inline", d, 16);
-  run<30>("v_pk_mul", d, 8);
   return 0;
 }
