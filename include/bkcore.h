@@ -350,6 +350,84 @@ int bkcore_woodbury_correct(const float *G, const float *U, const float *V, int6
                             float *out, void *workspace, size_t workspace_bytes, void *stream);
 size_t bkcore_woodbury_workspace_bytes(int64_t B, int64_t N, int64_t r);
 
+/*
+ * The operators of the mixing layer around the resolvent gate: layer norm, the short causal convolution and the selective
+ * scan of a selective mixer, sliding-window attention with sinks.  Element types BKCORE_F32 / BF16 / F16 (`dtype`, of all
+ * activations of a call); arithmetic, sums and states are float32.  Strides are in elements; the innermost dimension
+ * (channels, head dimension) has stride 1.  `lengths` is NULL or B ints on the device: positions at or behind a
+ * sequence's length are padding, which is never read; outputs and gradients there are zero (values outside 0..L are
+ * taken as the nearest of the two).  Workspaces need 16-byte alignment.
+ */
+
+/* Layer norm over D elements, rows of stride ldx: y = (x - mean) / sqrt(var + eps) * weight + bias, y contiguous.
+ * Replaces nn.LayerNorm in front of every block, behind the gate and in front of the head (src/models/resnet_bk.py:
+ * 243-244, src/models/phase7/hybrid_attention.py:55,143).  weight, bias: D values of param_dtype (BKCORE_F32 or dtype) or
+ * NULL.  stats: NULL, or 2 rows floats (means, then 1/sqrt(var + eps)) for the backward. */
+#define BKCORE_LAYER_NORM_MAX_DIM 16384
+int bkcore_layer_norm(const void *x, int64_t ldx, int dtype, const void *weight, const void *bias, int param_dtype,
+                      float eps, int64_t rows, int64_t D, void *y, float *stats, void *stream);
+/* dx (contiguous) and, unless NULL, grad_params: D floats of the weight's gradient, then D of the bias'.  Sums over rows
+ * in a fixed order.  With rows == 0 nothing is written. */
+size_t bkcore_layer_norm_backward_workspace_bytes(int64_t rows, int64_t D);
+int bkcore_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, int dtype, const void *weight,
+                               int param_dtype, const float *stats, int64_t rows, int64_t D, void *dx,
+                               float *grad_params, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Depthwise causal convolution over (B, L, C), K taps (2..4): y_t = act(bias + sum_k weight[c, k] x_{t-K+1+k}), act silu
+ * or none; y contiguous.  x in front of the first position comes from initial_state ((B, K-1, C) contiguous, dtype), or
+ * is zero.  final_state (same layout, may be NULL): the last K-1 inputs of each sequence. */
+#define BKCORE_CONV_MIN_WIDTH 2
+#define BKCORE_CONV_MAX_WIDTH 4
+int bkcore_causal_conv(const void *x, int64_t x_batch, int64_t x_time, int dtype, const void *weight, const void *bias,
+                       int param_dtype, const void *initial_state, const int *lengths, int64_t B, int64_t L, int64_t C,
+                       int64_t K, int silu, void *y, void *final_state, void *stream);
+/* dx (contiguous); grad_params (or NULL): (K + 1) C floats, K rows of C (the gradient of weight[:, k]) and the bias' row;
+ * grad_final_state, grad_initial_state: NULL or the states' layout. */
+size_t bkcore_causal_conv_backward_workspace_bytes(int64_t B, int64_t L, int64_t C, int64_t K);
+int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int64_t dy_time, const void *x, int64_t x_batch,
+                                int64_t x_time, int dtype, const void *weight, const void *bias, int param_dtype,
+                                const void *initial_state, const void *grad_final_state, const int *lengths, int64_t B,
+                                int64_t L, int64_t C, int64_t K, int silu, void *dx, float *grad_params,
+                                void *grad_initial_state, void *workspace, size_t workspace_bytes, void *stream);
+/* One token: x (B, C), y (B, C) contiguous; state (B, K-1, C) contiguous moves on by one position in place. */
+int bkcore_causal_conv_step(const void *x, int64_t x_batch, int dtype, void *state, const void *weight, const void *bias,
+                            int param_dtype, int64_t B, int64_t C, int64_t K, int silu, void *y, void *stream);
+
+/* Selective scan over (B, L, C) with N <= 64 states a channel:
+ *   d = softplus(delta + delta_bias) (softplus_delta != 0) or delta + delta_bias;
+ *   h_t = exp(d A) h_{t-1} + d x B_t;  y = (C_t . h_t + D x) silu(z)
+ * A (C, N), D (C), delta_bias (C) float32; Bm, Cm (B, L, N) shared by the channels; D, z, delta_bias may be NULL;
+ * y contiguous.  initial_state, final_state: (B, C, N) float32 or NULL.  checkpoints: NULL, or
+ * bkcore_selective_scan_checkpoint_bytes for the backward (16-byte aligned).  The workspace is needed when its size is
+ * not zero.  Takes the place of the causal accumulation of the reference's global path
+ * (src/models/phase1/ar_ssm_layer.py:517-525) where its decay depends on the input. */
+#define BKCORE_SCAN_MAX_STATE 64
+size_t bkcore_selective_scan_workspace_bytes(int64_t B, int64_t L, int64_t C, int64_t N);
+size_t bkcore_selective_scan_checkpoint_bytes(int64_t B, int64_t L, int64_t C, int64_t N);
+int bkcore_selective_scan(const void *x, int64_t x_batch, int64_t x_time, const void *delta, int64_t delta_batch,
+                          int64_t delta_time, const float *A, const void *Bm, int64_t B_batch, int64_t B_time,
+                          const void *Cm, int64_t C_batch, int64_t C_time, const float *D, const void *z, int64_t z_batch,
+                          int64_t z_time, const float *delta_bias, int softplus_delta, int dtype, const int *lengths,
+                          const float *initial_state, int64_t B, int64_t L, int64_t C, int64_t N, void *y,
+                          float *final_state, float *checkpoints, void *workspace, size_t workspace_bytes, void *stream);
+/* dx, grad_delta, dz (B, L, C) and dB, dC (B, L, N) contiguous, dtype; grad_params: C N floats of dA, C of dD, C of the
+ * delta bias' gradient; grad_final_state, grad_initial_state (B, C, N) float32 or NULL. */
+size_t bkcore_selective_scan_backward_workspace_bytes(int64_t B, int64_t L, int64_t C, int64_t N);
+int bkcore_selective_scan_backward(const void *dy, int64_t dy_batch, int64_t dy_time, const float *grad_final_state,
+                                   const void *x, int64_t x_batch, int64_t x_time, const void *delta,
+                                   int64_t delta_batch, int64_t delta_time, const float *A, const void *Bm,
+                                   int64_t B_batch, int64_t B_time, const void *Cm, int64_t C_batch, int64_t C_time,
+                                   const float *D, const void *z, int64_t z_batch, int64_t z_time,
+                                   const float *delta_bias, int softplus_delta, int dtype, const int *lengths,
+                                   const float *checkpoints, int64_t B, int64_t L, int64_t C, int64_t N, void *dx,
+                                   void *grad_delta, float *grad_params, void *dB, void *dC, void *dz,
+                                   float *grad_initial_state, void *workspace, size_t workspace_bytes, void *stream);
+/* One token: x, delta, z (B, C), Bm, Cm (B, N), y (B, C) contiguous; state (B, C, N) float32 is updated in place. */
+int bkcore_selective_scan_step(const void *x, int64_t x_batch, float *state, const void *delta, int64_t delta_batch,
+                               const float *A, const void *Bm, int64_t B_batch, const void *Cm, int64_t C_batch,
+                               const float *D, const void *z, int64_t z_batch, const float *delta_bias,
+                               int softplus_delta, int dtype, int64_t B, int64_t C, int64_t N, void *y, void *stream);
+
 /* Largest N bkcore_forward accepts. */
 int64_t bkcore_max_seq_len(void);
 

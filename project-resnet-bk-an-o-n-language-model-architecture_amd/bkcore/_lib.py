@@ -20,7 +20,7 @@ FLAG_ROW_UNITS_MUTE = 64
 FLAG_WHOLE_ROWS = 128
 FLAG_ROWS_UNCUT = 256      # diagnostics: one workgroup per row whatever the shape
 STATE_BYTES = 64
-ABI_VERSION = 18
+ABI_VERSION = 19
 EINVAL, ETOOLONG, ELAUNCH, EWORKSPACE, ETOOBIG = -1, -2, -3, -4, -5
 BWD_REFERENCE, BWD_BATCHED, BWD_SCAN_STABLE = 0, 1, 2
 NOALLOC_MAX_WORKSPACE = 8 << 20
@@ -31,6 +31,11 @@ EXPORTS = ("bkcore_forward", "bkcore_forward_clamped", "bkcore_forward_noalloc",
            "bkcore_layer_epilogue", "bkcore_layer_epilogue_backward", "bkcore_layer_epilogue_backward_workspace_bytes",
            "bkcore_layer_epilogue_clamped", "bkcore_layer_epilogue_backward_clamped", "bkcore_cumsum", "bkcore_woodbury_correct", "bkcore_woodbury_workspace_bytes",
            "bkcore_get_diag_complex", "bkcore_get_diag_complex_workspace_bytes",
+           "bkcore_layer_norm", "bkcore_layer_norm_backward", "bkcore_layer_norm_backward_workspace_bytes",
+           "bkcore_causal_conv", "bkcore_causal_conv_backward", "bkcore_causal_conv_backward_workspace_bytes",
+           "bkcore_causal_conv_step", "bkcore_selective_scan", "bkcore_selective_scan_workspace_bytes",
+           "bkcore_selective_scan_checkpoint_bytes", "bkcore_selective_scan_backward",
+           "bkcore_selective_scan_backward_workspace_bytes", "bkcore_selective_scan_step",
            "bkcore_max_seq_len", "bkcore_forward_plan", "bkcore_last_hip_error",
            "bkcore_error_string", "bkcore_abi_version")
 
@@ -107,6 +112,28 @@ def load():
     L.bkcore_get_diag_complex.restype = i32
     L.bkcore_get_diag_complex_workspace_bytes.argtypes = [i64, i64]
     L.bkcore_get_diag_complex_workspace_bytes.restype = ctypes.c_size_t
+    sz = ctypes.c_size_t
+    for name, args in {
+            "layer_norm": [vp, i64, i32, vp, vp, i32, f32, i64, i64, vp, vp, vp],
+            "layer_norm_backward": [vp, i64, vp, i64, i32, vp, i32, vp, i64, i64, vp, vp, vp, sz, vp],
+            "causal_conv": [vp, i64, i64, i32, vp, vp, i32, vp, vp, i64, i64, i64, i64, i32, vp, vp, vp],
+            "causal_conv_backward": [vp, i64, i64, vp, i64, i64, i32, vp, vp, i32, vp, vp, vp, i64, i64, i64, i64, i32, vp,
+                                     vp, vp, vp, sz, vp],
+            "causal_conv_step": [vp, i64, i32, vp, vp, vp, i32, i64, i64, i64, i32, vp, vp],
+            "selective_scan": [vp, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp, i32, i32, vp,
+                               vp, i64, i64, i64, i64, vp, vp, vp, vp, sz, vp],
+            "selective_scan_backward": [vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, vp, vp,
+                                        i64, i64, vp, i32, i32, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp,
+                                        sz, vp],
+            "selective_scan_step": [vp, i64, vp, vp, i64, vp, vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i64, i64, i64, vp,
+                                    vp]}.items():
+        fn = getattr(L, "bkcore_" + name)
+        fn.argtypes, fn.restype = args, i32
+    for name, n in {"layer_norm_backward_workspace_bytes": 2, "causal_conv_backward_workspace_bytes": 4,
+                    "selective_scan_workspace_bytes": 4, "selective_scan_checkpoint_bytes": 4,
+                    "selective_scan_backward_workspace_bytes": 4}.items():
+        fn = getattr(L, "bkcore_" + name)
+        fn.argtypes, fn.restype = [i64] * n, sz
     L.bkcore_max_seq_len.restype = i64
     L.bkcore_forward_plan.argtypes = [i64, i64, i32, ctypes.c_uint, i32, ctypes.POINTER(ctypes.c_int)]
     L.bkcore_forward_plan.restype = i32

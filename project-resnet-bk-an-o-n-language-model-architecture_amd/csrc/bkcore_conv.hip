@@ -1,0 +1,343 @@
+// The short causal convolution of a selective mixer (depthwise, K = 2..4 taps, channels innermost), forward, backward and
+// for single tokens.
+//   pre_t = bias + sum_k w_k x_{t-K+1+k},  y_t = pre_t or silu(pre_t);  x at t < 0 is the carried state, or zero
+//   g_t = dy_t act'(pre_t);  dx_t = sum_k w_k g_{t+K-1-k};  dw_k = sum g_t x_{t-K+1+k};  db = sum g_t
+// Positions at or behind a sequence's length are padding: they are never read, y and dx there are zero.
+// HBM-bound: 2 e bytes an element forward, 3 e backward.  A thread holds V neighbouring channels (one 16-byte access a
+// position) and walks TL positions with the last K - 1 inputs in registers; only the K - 1 positions in front of its
+// stretch are read twice, from cache.  Arithmetic and sums are float32.
+#include "bkcore_types.h"
+
+namespace {
+using namespace bk;
+
+constexpr int FWD_TL = 16;  // positions a thread walks forward: 3 of 19 reads are repeated
+constexpr int BWD_TL = 32;  // ... and backward
+constexpr int BWD_SEGS = 8; // stretches of one workgroup, joined before the partial sums are written
+constexpr int BWD_CH = 32;  // channel vectors of one workgroup
+
+struct ConvArgs {
+  const void *x, *w, *bias, *init, *dy, *dfinal;
+  void *y, *final_state, *dx, *dinit;
+  float *part;
+  const int *lengths;
+  long xb, xt, dyb, dyt;  // strides of x and dy in elements
+  int B, L, C, param_f32, silu;
+};
+
+__device__ __forceinline__ int row_length(const int *lengths, int b, int L) {
+  if (!lengths) return L;
+  const int n = lengths[b];
+  return n < 0 ? 0 : n > L ? L : n;
+}
+
+// x_t of sequence b for V channels from c: the carried state for t < 0, zero where there is none or behind the length.
+template <typename T, int K, int V>
+__device__ __forceinline__ void input_at(const ConvArgs &a, int b, long t, int len, int c, float (&v)[V]) {
+  if (t >= 0 && t < len) {
+    load_vec<T, V>((const T *)a.x + b * a.xb + t * a.xt + c, v);
+  } else if (t < 0 && a.init) {
+    load_vec<T, V>((const T *)a.init + ((long)b * (K - 1) + (t + K - 1)) * a.C + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.0f;
+  }
+}
+
+template <typename T, int K, int V>
+__device__ __forceinline__ void load_taps(const ConvArgs &a, int c, float (&w)[K][V], float (&bias)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float t[1];
+      load_param<T, 1>(a.w, a.param_f32, (long)(c + i) * K + k, t);
+      w[k][i] = t[0];
+    }
+    bias[i] = 0.0f;
+  }
+  if (a.bias) load_param<T, V>(a.bias, a.param_f32, c, bias);
+}
+
+template <typename T, int K, int V>
+__global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int nvec) {
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)a.B * nseg * nvec) return;
+  const int c = (int)(id % nvec) * V;
+  const long r = id / nvec;
+  const int seg = (int)(r % nseg), b = (int)(r / nseg);
+  const int len = row_length(a.lengths, b, a.L);
+  float w[K][V], bias[V], h[K][V];
+  load_taps<T, K, V>(a, c, w, bias);
+  const long t0 = (long)seg * FWD_TL, t1 = t0 + FWD_TL < a.L ? t0 + FWD_TL : a.L;
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) input_at<T, K, V>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+  T *y = (T *)a.y + ((long)b * a.L) * a.C + c;
+#pragma unroll 4
+  for (long t = t0; t < t1; ++t) {
+    input_at<T, K, V>(a, b, t, len, c, h[K - 1]);
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float s = bias[i];
+#pragma unroll
+      for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
+      if (a.silu) s = s * sigmoid(s);
+      o[i] = t < len ? s : 0.0f;
+    }
+    store_vec<T, V>(y + t * a.C, o);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[k][i] = h[k + 1][i];
+  }
+  if (a.final_state && seg == 0) {  // the last K - 1 inputs, the carried ones among them for a short sequence
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      float v[V];
+      input_at<T, K, V>(a, b, (long)len - (K - 1) + j, len, c, v);
+      store_vec<T, V>((T *)a.final_state + ((long)b * (K - 1) + j) * a.C + c, v);
+    }
+  }
+}
+
+// One workgroup: 32 channel vectors x 8 stretches of 32 positions of one sequence.  part: one row of (K + 1) C floats
+// per (sequence, workgroup along time): K rows of the weights' sums, then the bias'.
+template <typename T, int K, int V>
+__global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(ConvArgs a, int nblk, int cblk) {
+  __shared__ float join[BWD_SEGS][BWD_CH][V + 1];
+  const int cv = threadIdx.x % BWD_CH, sg = threadIdx.x / BWD_CH;
+  const int cb = blockIdx.x % cblk;
+  const long stretch = blockIdx.x / cblk;  // sequence and workgroup along time
+  const int b = (int)(stretch / nblk), tb = (int)(stretch % nblk);
+  const int c = (cb * BWD_CH + cv) * V;
+  const bool live = c < a.C;
+  const int len = row_length(a.lengths, b, a.L);
+  float dw[K][V], db[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    db[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) dw[k][i] = 0.0f;
+  }
+  const long t0 = ((long)tb * BWD_SEGS + sg) * BWD_TL;
+  const long t1 = t0 + BWD_TL < a.L ? t0 + BWD_TL : a.L;
+  if (live && t0 < a.L) {
+    float w[K][V], bias[V], h[K][V], g[K][V];  // h: x_{t-K+1..t};  g: g_{t-K+1..t}
+    load_taps<T, K, V>(a, c, w, bias);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) input_at<T, K, V>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+    const T *dy = (const T *)a.dy + b * a.dyb + c;
+    T *dx = (T *)a.dx + (long)b * a.L * a.C + c;
+    // dx of position t - K + 1 is complete once g_t is known; the first stretch also gives the carried state's gradient
+    for (long t = t0; t < t1 + K - 1; ++t) {
+      if (t < len) {
+        input_at<T, K, V>(a, b, t, len, c, h[K - 1]);
+        float d[V];
+        load_vec<T, V>(dy + t * a.dyt, d);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (a.silu) {
+            float s = bias[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
+            const float sg1 = sigmoid(s);
+            d[i] *= sg1 * fmaf(s, 1.0f - sg1, 1.0f);
+          }
+          g[K - 1][i] = d[i];
+          if (t < t1) {
+            db[i] += d[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d[i], h[k][i], dw[k][i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[K - 1][i] = g[K - 1][i] = 0.0f;
+      }
+      const long p = t - (K - 1);  // the position that is complete now
+      if (p >= t0 || (t0 == 0 && a.dinit)) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float s = 0.0f;
+#pragma unroll
+          for (int k = 0; k < K; ++k) s = fmaf(w[k][i], g[K - 1 - k][i], s);
+          o[i] = s;
+        }
+        const long j = p - ((long)len - (K - 1));  // its place in the final state
+        if (a.dfinal && j >= 0 && p < len) {
+          float f[V];
+          load_vec<T, V>((const T *)a.dfinal + ((long)b * (K - 1) + j) * a.C + c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] += f[i];
+        }
+        if (p >= t0)
+          store_vec<T, V>(dx + p * a.C, o);
+        else
+          store_vec<T, V>((T *)a.dinit + ((long)b * (K - 1) + (p + K - 1)) * a.C + c, o);
+      }
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          h[k][i] = h[k + 1][i];
+          g[k][i] = g[k + 1][i];
+        }
+    }
+  }
+  if (!a.part) return;
+  float *out = a.part + stretch * (K + 1) * a.C;
+#pragma unroll
+  for (int k = 0; k <= K; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) join[sg][cv][i] = k < K ? dw[k < K ? k : 0][i] : db[i];
+    __syncthreads();
+    for (int j = threadIdx.x; j < BWD_CH * V; j += BWD_CH * BWD_SEGS) {
+      const int col = cb * BWD_CH * V + j;
+      if (col < a.C) {
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < BWD_SEGS; ++q) s += join[q][j / V][j % V];
+        out[(long)k * a.C + col] = s;
+      }
+    }
+  }
+}
+
+// One token: the window is the state and the new input; the state moves on by one position in place.
+template <typename T, int K, int V>
+__global__ __launch_bounds__(256) void bk_conv_step_kernel(ConvArgs a, T *__restrict__ state, int nvec) {
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)a.B * nvec) return;
+  const int c = (int)(id % nvec) * V, b = (int)(id / nvec);
+  float w[K][V], bias[V], h[K][V];
+  load_taps<T, K, V>(a, c, w, bias);
+  T *st = state + (long)b * (K - 1) * a.C + c;
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) load_vec<T, V>(st + (long)k * a.C, h[k]);
+  load_vec<T, V>((const T *)a.x + b * a.xb + c, h[K - 1]);
+  float o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float s = bias[i];
+#pragma unroll
+    for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
+    o[i] = a.silu ? s * sigmoid(s) : s;
+  }
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) store_vec<T, V>(st + (long)k * a.C, h[k + 1]);
+  store_vec<T, V>((T *)a.y + (long)b * a.C + c, o);
+}
+
+int check(int dtype, int param_dtype, int64_t B, int64_t L, int64_t C, int64_t K) {
+  if (!elem_size(dtype) || (param_dtype != BKCORE_F32 && param_dtype != dtype)) return BKCORE_EINVAL;
+  if (B < 0 || L < 0 || C < 0 || K < BKCORE_CONV_MIN_WIDTH || K > BKCORE_CONV_MAX_WIDTH) return BKCORE_EINVAL;
+  if (B > (1 << 24) || L > (1 << 30) || C > (1 << 24)) return BKCORE_EINVAL;
+  return BKCORE_OK;
+}
+
+inline int64_t backward_blocks(int64_t L) { return (L + BWD_TL * BWD_SEGS - 1) / (BWD_TL * BWD_SEGS); }
+
+}  // namespace
+
+#define BK_CONV_K(K, LAUNCH, V)             \
+  do {                                      \
+    if ((K) == 2) LAUNCH(2, V);             \
+    else if ((K) == 3) LAUNCH(3, V);        \
+    else LAUNCH(4, V);                      \
+  } while (0)
+
+extern "C" int bkcore_causal_conv(const void *x, int64_t x_batch, int64_t x_time, int dtype, const void *weight,
+                                  const void *bias, int param_dtype, const void *initial_state, const int *lengths,
+                                  int64_t B, int64_t L, int64_t C, int64_t K, int silu, void *y, void *final_state,
+                                  void *stream) {
+  const int rc = check(dtype, param_dtype, B, L, C, K);
+  if (rc) return rc;
+  if (B == 0 || C == 0 || (L == 0 && !final_state)) return BKCORE_OK;
+  if ((L > 0 && (!x || !y)) || !weight) return BKCORE_EINVAL;
+  const int v = 16 / elem_size(dtype);
+  const bool vec = C % v == 0 && x_batch % v == 0 && x_time % v == 0 && aligned16(x) && aligned16(y) &&
+                   aligned16(initial_state) && aligned16(final_state);
+  ConvArgs a{};
+  a.x = x; a.w = weight; a.bias = bias; a.init = initial_state; a.y = y; a.final_state = final_state;
+  a.lengths = lengths; a.xb = x_batch; a.xt = x_time; a.B = (int)B; a.L = (int)L; a.C = (int)C;
+  a.param_f32 = param_dtype == BKCORE_F32; a.silu = silu != 0;
+  const int64_t nseg = L > 0 ? (L + FWD_TL - 1) / FWD_TL : 1, nvec = vec ? C / v : C;
+  const int64_t blocks = (B * nseg * nvec + 255) / 256;
+  if (blocks > 2147483647LL) return BKCORE_EINVAL;
+#define BK_CONV(K_, V_)                                                                                            \
+  hipLaunchKernelGGL((bk_conv_kernel<T, K_, V_>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, (int)nseg, \
+                     (int)nvec)
+  if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, (int)(16 / sizeof(T))));
+  else BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, 1));
+#undef BK_CONV
+  return launch_status();
+}
+
+extern "C" size_t bkcore_causal_conv_backward_workspace_bytes(int64_t B, int64_t L, int64_t C, int64_t K) {
+  if (B <= 0 || L <= 0 || C <= 0 || K <= 0) return 0;
+  return (size_t)B * (size_t)backward_blocks(L) * (size_t)(K + 1) * (size_t)C * sizeof(float);
+}
+
+extern "C" int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int64_t dy_time, const void *x,
+                                           int64_t x_batch, int64_t x_time, int dtype, const void *weight,
+                                           const void *bias, int param_dtype, const void *initial_state,
+                                           const void *grad_final_state, const int *lengths, int64_t B, int64_t L,
+                                           int64_t C, int64_t K, int silu, void *dx, float *grad_params,
+                                           void *grad_initial_state, void *workspace, size_t workspace_bytes,
+                                           void *stream) {
+  const int rc = check(dtype, param_dtype, B, L, C, K);
+  if (rc) return rc;
+  if (B == 0 || L == 0 || C == 0) return BKCORE_OK;
+  if (!dy || !x || !weight || !dx || (grad_initial_state && !initial_state)) return BKCORE_EINVAL;
+  if (grad_params && (!workspace || workspace_bytes < bkcore_causal_conv_backward_workspace_bytes(B, L, C, K)))
+    return BKCORE_EWORKSPACE;
+  const int v = 16 / elem_size(dtype);
+  const bool vec = C % v == 0 && x_batch % v == 0 && x_time % v == 0 && dy_batch % v == 0 && dy_time % v == 0 &&
+                   aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(initial_state) &&
+                   aligned16(grad_initial_state) && aligned16(grad_final_state);
+  ConvArgs a{};
+  a.x = x; a.w = weight; a.bias = bias; a.init = initial_state; a.dy = dy; a.dfinal = grad_final_state;
+  a.dx = dx; a.dinit = grad_initial_state; a.part = grad_params ? (float *)workspace : nullptr; a.lengths = lengths;
+  a.xb = x_batch; a.xt = x_time; a.dyb = dy_batch; a.dyt = dy_time; a.B = (int)B; a.L = (int)L; a.C = (int)C;
+  a.param_f32 = param_dtype == BKCORE_F32; a.silu = silu != 0;
+  const int64_t nblk = backward_blocks(L), nvec = vec ? C / v : C, cblk = (nvec + BWD_CH - 1) / BWD_CH;
+  if (B * nblk * cblk > 2147483647LL) return BKCORE_EINVAL;
+#define BK_CONV(K_, V_)                                                                                              \
+  hipLaunchKernelGGL((bk_conv_backward_kernel<T, K_, V_>), dim3((unsigned)(B * nblk * cblk)), dim3(BWD_CH * BWD_SEGS), \
+                     0, (hipStream_t)stream, a, (int)nblk, (int)cblk)
+  if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, (int)(16 / sizeof(T))));
+  else BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, 1));
+#undef BK_CONV
+  if (grad_params) bkcore_internal_sum_parts((const float *)workspace, B * nblk, (K + 1) * C, grad_params, stream);
+  return launch_status();
+}
+
+extern "C" int bkcore_causal_conv_step(const void *x, int64_t x_batch, int dtype, void *state, const void *weight,
+                                       const void *bias, int param_dtype, int64_t B, int64_t C, int64_t K, int silu,
+                                       void *y, void *stream) {
+  const int rc = check(dtype, param_dtype, B, 1, C, K);
+  if (rc) return rc;
+  if (B == 0 || C == 0) return BKCORE_OK;
+  if (!x || !state || !weight || !y) return BKCORE_EINVAL;
+  const int v = 16 / elem_size(dtype);
+  const bool vec = C % v == 0 && x_batch % v == 0 && aligned16(x) && aligned16(y) && aligned16(state);
+  ConvArgs a{};
+  a.x = x; a.w = weight; a.bias = bias; a.y = y; a.xb = x_batch; a.B = (int)B; a.L = 1; a.C = (int)C;
+  a.param_f32 = param_dtype == BKCORE_F32; a.silu = silu != 0;
+  const int64_t nvec = vec ? C / v : C, blocks = (B * nvec + 255) / 256;
+  if (blocks > 2147483647LL) return BKCORE_EINVAL;
+#define BK_CONV(K_, V_)                                                                                              \
+  hipLaunchKernelGGL((bk_conv_step_kernel<T, K_, V_>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, \
+                     (T *)state, (int)nvec)
+  if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, (int)(16 / sizeof(T))));
+  else BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, 1));
+#undef BK_CONV
+  return launch_status();
+}

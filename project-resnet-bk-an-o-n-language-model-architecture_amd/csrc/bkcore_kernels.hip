@@ -1960,7 +1960,7 @@ int bkcore_forward_plan(int64_t B, int64_t N, int in_dtype, unsigned flags, int 
 }
 int bkcore_last_hip_error(void) { return g_last_hip_error; }
 void bkcore_internal_set_hip_error(int code) { g_last_hip_error = code; }
-int bkcore_abi_version(void) { return 18; }
+int bkcore_abi_version(void) { return 19; }
 
 const char *bkcore_error_string(int code) {
   switch (code) {
