@@ -381,7 +381,7 @@ int bkcore_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int6
 int bkcore_causal_conv(const void *x, int64_t x_batch, int64_t x_time, int dtype, const void *weight, const void *bias,
                        int param_dtype, const void *initial_state, const int *lengths, int64_t B, int64_t L, int64_t C,
                        int64_t K, int silu, void *y, void *final_state, void *stream);
-/* dx (contiguous); grad_params (or NULL): (K + 1) C floats, K rows of C (the gradient of weight[:, k]) and the bias' row;
+/* dx (contiguous); grad_params (or NULL): (K + 1) C floats, the weight's gradient (C, K), then the bias';
  * grad_final_state, grad_initial_state: NULL or the states' layout. */
 size_t bkcore_causal_conv_backward_workspace_bytes(int64_t B, int64_t L, int64_t C, int64_t K);
 int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int64_t dy_time, const void *x, int64_t x_batch,

@@ -4,6 +4,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .bk_core import _on_device as on_device
 
 DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -77,15 +78,19 @@ def lengths_arg(what: str, lengths: torch.Tensor | None, x: torch.Tensor, batch:
     return lengths.clamp(0, longest).to(torch.int32)
 
 
+def once_only(what: str) -> None:
+    """First line of a backward pass: gradient mode is on there only under create_graph."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"bkcore: {what} has first derivatives only (create_graph is not supported)")
+
+
 def ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    """Scratch memory of one call, from the allocator: its stream order keeps calls on different streams and captured
-    graphs apart."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def strides(t: torch.Tensor | None) -> tuple:
+    """The two outer strides of a three-dimensional operand."""
+    return (0, 0) if t is None else t.stride()[:2]
 
 
-def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+stream = torch._C._cuda_getCurrentRawStream     # of a device index: the handle alone, without a Stream object around it

@@ -40,6 +40,7 @@ EXPORTS = ("bkcore_forward", "bkcore_forward_clamped", "bkcore_forward_noalloc",
            "bkcore_error_string", "bkcore_abi_version")
 
 _lib = None
+_held = None
 
 
 def load():
@@ -51,6 +52,27 @@ def load():
             f"bkcore: {LIB_PATH} not found. Build it with `make -C <package>/csrc` (hipcc --offload-arch=gfx950); "
             "there is no CPU fallback for this operator.")
     L = ctypes.CDLL(LIB_PATH)
+    _declare(L)
+    if L.bkcore_abi_version() != ABI_VERSION:
+        raise RuntimeError(f"bkcore: ABI version mismatch (library {L.bkcore_abi_version()}, wrapper {ABI_VERSION})")
+    _lib = L
+    return L
+
+
+def load_held():
+    """The library with the interpreter lock kept during a call, for the layer operators: their calls check arguments,
+    launch and return, and in a backward pass, which runs on the autograd engine's thread, giving the lock away and
+    fetching it back costs more than the call (a layer norm step 148 -> 96 us on the host)."""
+    global _held
+    if _held is None:
+        load()
+        L = ctypes.PyDLL(LIB_PATH)
+        _declare(L)
+        _held = L
+    return _held
+
+
+def _declare(L):
     vp, i64, i32, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
     L.bkcore_forward.argtypes = [vp, i64, vp, i64, vp, i64, i32, vp, f32, f32, i64, i64, vp, vp, vp, ctypes.c_size_t,
                                  vp, ctypes.c_uint, vp]
@@ -141,10 +163,6 @@ def load():
     L.bkcore_error_string.argtypes = [i32]
     L.bkcore_error_string.restype = ctypes.c_char_p
     L.bkcore_abi_version.restype = i32
-    if L.bkcore_abi_version() != ABI_VERSION:
-        raise RuntimeError(f"bkcore: ABI version mismatch (library {L.bkcore_abi_version()}, wrapper {ABI_VERSION})")
-    _lib = L
-    return L
 
 
 def check(rc, what):

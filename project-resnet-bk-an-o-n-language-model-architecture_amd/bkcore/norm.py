@@ -4,7 +4,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _layer_ops as ops
 from . import _lib
@@ -15,19 +14,21 @@ MAX_DIM = 16384   # BKCORE_LAYER_NORM_MAX_DIM
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
-        L = _lib.load()
         D = x.shape[-1]
-        x2 = ops.inner(x.reshape(-1, D))
+        x2 = ops.inner(x if x.dim() == 2 else x.reshape(-1, D))
         rows = x2.shape[0]
         w = None if weight is None else weight.contiguous()
         b = None if bias is None else bias.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
-        param = ops.DTYPES[(w if w is not None else b if b is not None else x2).dtype]
-        with torch.cuda.device(x.device):
-            rc = L.bkcore_layer_norm(ops.ptr(x2), x2.stride(0), ops.DTYPES[x.dtype], ops.ptr(w), ops.ptr(b), param, eps,
-                                     rows, D, ops.ptr(y), ops.ptr(stats), ops.stream())
-        _lib.check(rc, "bkcore_layer_norm")
+        dev = x.device
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=dev) if keep else None
+        p = w if w is not None else b if b is not None else x2
+        with ops.on_device(dev):
+            rc = _lib.load_held().bkcore_layer_norm(
+                x2.data_ptr(), x2.stride(0), ops.DTYPES[x.dtype], ops.ptr(w), ops.ptr(b), ops.DTYPES[p.dtype], eps, rows, D,
+                y.data_ptr(), ops.ptr(stats), ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_layer_norm")
         if keep:
             ctx.save_for_backward(x2, w, stats)
             ctx.bk_bias = None if bias is None else bias.dtype
@@ -35,27 +36,32 @@ class _LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        L = _lib.load()
+        ops.once_only("layer_norm")
         x2, w, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         rows, D = x2.shape
-        want = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        g2 = ops.inner(dy.reshape(-1, D))
-        dx = torch.empty(rows, D, dtype=x2.dtype, device=x2.device)
-        gp = torch.empty(2, D, dtype=torch.float32, device=x2.device) if want else None
-        if want and rows == 0:
-            gp.zero_()
-        with torch.cuda.device(x2.device):
-            nbytes = int(L.bkcore_layer_norm_backward_workspace_bytes(rows, D)) if want else 0
-            ws = ops.scratch(nbytes, x2.device)
-            rc = L.bkcore_layer_norm_backward(ops.ptr(g2), g2.stride(0), ops.ptr(x2), x2.stride(0), ops.DTYPES[x2.dtype],
-                                              ops.ptr(w), ops.DTYPES[(x2 if w is None else w).dtype], ops.ptr(stats), rows,
-                                              D, ops.ptr(dx), ops.ptr(gp), ops.ptr(ws), nbytes, ops.stream())
-        _lib.check(rc, "bkcore_layer_norm_backward")
-        dw = gp[0].to(w.dtype) if ctx.needs_input_grad[1] else None
-        db = gp[1].to(ctx.bk_bias) if ctx.needs_input_grad[2] else None
-        return dx.reshape(ctx.bk_shape) if ctx.needs_input_grad[0] else None, dw, db, None, None
+        dev = x2.device
+        g2 = ops.inner(dy if dy.dim() == 2 else dy.reshape(-1, D))
+        dx = torch.empty(rows, D, dtype=x2.dtype, device=dev)
+        L = _lib.load_held()
+        gp = ws = None
+        nbytes = 0
+        if need_w or need_b:
+            nbytes = L.bkcore_layer_norm_backward_workspace_bytes(rows, D)
+            gp = torch.empty(2 * D, dtype=torch.float32, device=dev)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            if rows == 0:
+                gp.zero_()
+        with ops.on_device(dev):
+            rc = L.bkcore_layer_norm_backward(
+                g2.data_ptr(), g2.stride(0), x2.data_ptr(), x2.stride(0), ops.DTYPES[x2.dtype], ops.ptr(w),
+                ops.DTYPES[(x2 if w is None else w).dtype], stats.data_ptr(), rows, D, dx.data_ptr(), ops.ptr(gp), ops.ptr(ws), nbytes,
+                ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_layer_norm_backward")
+        return (dx.view(ctx.bk_shape) if need_x else None, gp[:D].to(w.dtype) if need_w else None,
+                gp[D:].to(ctx.bk_bias) if need_b else None, None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,

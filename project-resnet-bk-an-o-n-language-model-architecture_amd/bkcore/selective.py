@@ -7,7 +7,6 @@ never read, outputs and gradients there are zero, and a returned state is the on
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _layer_ops as ops
 from . import _lib
@@ -37,20 +36,21 @@ def _conv_params(what, x, weight, bias):
 class _CausalConvFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, silu, keep, want_state):
-        L = _lib.load()
         x = ops.inner(x)
         w = weight.contiguous()
         b = None if bias is None else bias.contiguous()
         st = None if state is None else state.contiguous()
         B, T, C = x.shape
         K = w.shape[1]
-        y = torch.empty(B, T, C, dtype=x.dtype, device=x.device)
-        final = torch.empty(B, K - 1, C, dtype=x.dtype, device=x.device) if want_state else None
-        with torch.cuda.device(x.device):
-            rc = L.bkcore_causal_conv(ops.ptr(x), x.stride(0), x.stride(1), ops.DTYPES[x.dtype], ops.ptr(w), ops.ptr(b),
-                                      ops.DTYPES[w.dtype], ops.ptr(st), ops.ptr(lengths), B, T, C, K, silu, ops.ptr(y),
-                                      ops.ptr(final), ops.stream())
-        _lib.check(rc, "bkcore_causal_conv")
+        dev = x.device
+        y = torch.empty(B, T, C, dtype=x.dtype, device=dev)
+        final = torch.empty(B, K - 1, C, dtype=x.dtype, device=dev) if want_state else None
+        with ops.on_device(dev):
+            rc = _lib.load_held().bkcore_causal_conv(
+                x.data_ptr(), *ops.strides(x), ops.DTYPES[x.dtype], w.data_ptr(), ops.ptr(b), ops.DTYPES[w.dtype],
+                ops.ptr(st), ops.ptr(lengths), B, T, C, K, silu, y.data_ptr(), ops.ptr(final), ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_causal_conv")
         if keep:
             ctx.save_for_backward(x, w, b, st, lengths)
             ctx.bk_silu = silu
@@ -58,36 +58,38 @@ class _CausalConvFunction(torch.autograd.Function):
         return (y, final) if want_state else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dfinal=None):
-        L = _lib.load()
+        ops.once_only("causal_conv")
         x, w, b, st, lengths = ctx.saved_tensors
+        need_x, need_w, need_b, need_st = ctx.needs_input_grad[:4]
         B, T, C = x.shape
         K = w.shape[1]
         dev = x.device
         dy = torch.zeros(B, T, C, dtype=x.dtype, device=dev) if dy is None else ops.inner(dy)
         dfinal = None if dfinal is None else dfinal.contiguous()
         dx = torch.empty(B, T, C, dtype=x.dtype, device=dev)
-        want = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        gp = torch.empty(K + 1, C, dtype=torch.float32, device=dev) if want else None
-        dst = torch.empty_like(st) if st is not None and ctx.needs_input_grad[3] else None
+        dst = torch.empty_like(st) if st is not None and need_st else None
+        L = _lib.load_held()
+        gp = ws = None
+        nbytes = 0
+        if need_w or need_b:
+            gp = torch.empty(C * (K + 1), dtype=torch.float32, device=dev)
+            nbytes = L.bkcore_causal_conv_backward_workspace_bytes(B, T, C, K)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         if B == 0 or T == 0 or C == 0:       # nothing runs: no position, and the state passes through unchanged
-            if want:
+            if gp is not None:
                 gp.zero_()
             if dst is not None:
                 dst.zero_() if dfinal is None else dst.copy_(dfinal)
-        with torch.cuda.device(dev):
-            nbytes = int(L.bkcore_causal_conv_backward_workspace_bytes(B, T, C, K)) if want else 0
-            ws = ops.scratch(nbytes, dev)
-            rc = L.bkcore_causal_conv_backward(ops.ptr(dy), dy.stride(0), dy.stride(1), ops.ptr(x), x.stride(0),
-                                               x.stride(1), ops.DTYPES[x.dtype], ops.ptr(w), ops.ptr(b),
-                                               ops.DTYPES[w.dtype], ops.ptr(st), ops.ptr(dfinal), ops.ptr(lengths), B, T, C,
-                                               K, ctx.bk_silu, ops.ptr(dx), ops.ptr(gp), ops.ptr(dst), ops.ptr(ws), nbytes,
-                                               ops.stream())
-        _lib.check(rc, "bkcore_causal_conv_backward")
-        dw = gp[:K].t().to(w.dtype).contiguous() if ctx.needs_input_grad[1] else None
-        db = gp[K].to(w.dtype) if ctx.needs_input_grad[2] else None
-        return dx if ctx.needs_input_grad[0] else None, dw, db, dst, None, None, None, None
+        with ops.on_device(dev):
+            rc = L.bkcore_causal_conv_backward(
+                dy.data_ptr(), *ops.strides(dy), x.data_ptr(), *ops.strides(x), ops.DTYPES[x.dtype], w.data_ptr(), ops.ptr(b),
+                ops.DTYPES[w.dtype], ops.ptr(st), ops.ptr(dfinal), ops.ptr(lengths), B, T, C, K, ctx.bk_silu, dx.data_ptr(),
+                ops.ptr(gp), ops.ptr(dst), ops.ptr(ws), nbytes, ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_causal_conv_backward")
+        return (dx if need_x else None, gp[:C * K].view(C, K).to(w.dtype) if need_w else None,
+                gp[C * K:].to(w.dtype) if need_b else None, dst, None, None, None, None)
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -117,7 +119,6 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     what = "causal_conv_step"
     if x.dim() != 2:
         raise ValueError(f"bkcore: {what}: x is (B, C), got {tuple(x.shape)}")
-    L = _lib.load()
     K = _conv_params(what, x, weight, bias)
     B, C = x.shape
     ops.need_device(x, state)
@@ -129,11 +130,14 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     x = ops.inner(x)
     w = weight.contiguous()
     b = None if bias is None else bias.contiguous()
-    y = torch.empty(B, C, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = L.bkcore_causal_conv_step(ops.ptr(x), x.stride(0), ops.DTYPES[x.dtype], ops.ptr(state), ops.ptr(w), ops.ptr(b),
-                                       ops.DTYPES[w.dtype], B, C, K, silu, ops.ptr(y), ops.stream())
-    _lib.check(rc, "bkcore_causal_conv_step")
+    dev = x.device
+    y = torch.empty(B, C, dtype=x.dtype, device=dev)
+    with ops.on_device(dev):
+        rc = _lib.load_held().bkcore_causal_conv_step(
+            x.data_ptr(), x.stride(0), ops.DTYPES[x.dtype], state.data_ptr(), w.data_ptr(), ops.ptr(b), ops.DTYPES[w.dtype],
+            B, C, K, silu, y.data_ptr(), ops.stream(dev.index))
+    if rc:
+        _lib.check(rc, "bkcore_causal_conv_step")
     return y
 
 
@@ -154,65 +158,69 @@ def _scan_params(what, x, A, D, delta_bias):
 class _SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, A, Bm, Cm, D, z, bias, state, lengths, softplus, keep, want_state):
-        L = _lib.load()
-        x, delta, Bm, Cm, z = (ops.inner(t) for t in (x, delta, Bm, Cm, z))
-        A, D, bias, state = (None if t is None else t.contiguous() for t in (A, D, bias, state))
+        x, delta, Bm, Cm, z = ops.inner(x), ops.inner(delta), ops.inner(Bm), ops.inner(Cm), ops.inner(z)
+        A = A.contiguous()
+        D, bias, state = (None if t is None else t.contiguous() for t in (D, bias, state))
         B, T, C = x.shape
         N = A.shape[1]
         dev = x.device
+        L = _lib.load_held()
         y = torch.empty(B, T, C, dtype=x.dtype, device=dev)
         final = torch.empty(B, C, N, dtype=torch.float32, device=dev) if want_state else None
         if final is not None and T == 0:
             final.zero_() if state is None else final.copy_(state)
-        with torch.cuda.device(dev):
-            ckpt = ops.scratch(int(L.bkcore_selective_scan_checkpoint_bytes(B, T, C, N)), dev) if keep else None
-            nbytes = int(L.bkcore_selective_scan_workspace_bytes(B, T, C, N))
-            ws = ops.scratch(nbytes, dev)
-            rc = L.bkcore_selective_scan(ops.ptr(x), x.stride(0), x.stride(1), ops.ptr(delta), delta.stride(0),
-                                         delta.stride(1), ops.ptr(A), ops.ptr(Bm), Bm.stride(0), Bm.stride(1), ops.ptr(Cm),
-                                         Cm.stride(0), Cm.stride(1), ops.ptr(D), ops.ptr(z), 0 if z is None else z.stride(0),
-                                         0 if z is None else z.stride(1), ops.ptr(bias), softplus, ops.DTYPES[x.dtype],
-                                         ops.ptr(lengths), ops.ptr(state), B, T, C, N, ops.ptr(y), ops.ptr(final),
-                                         ops.ptr(ckpt), ops.ptr(ws), nbytes, ops.stream())
-        _lib.check(rc, "bkcore_selective_scan")
+        ckpt = None
+        if keep:
+            ckpt = torch.empty(L.bkcore_selective_scan_checkpoint_bytes(B, T, C, N), dtype=torch.uint8, device=dev)
+        nbytes = L.bkcore_selective_scan_workspace_bytes(B, T, C, N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with ops.on_device(dev):
+            rc = L.bkcore_selective_scan(
+                x.data_ptr(), *ops.strides(x), delta.data_ptr(), *ops.strides(delta), A.data_ptr(), Bm.data_ptr(),
+                *ops.strides(Bm), Cm.data_ptr(), *ops.strides(Cm), ops.ptr(D), ops.ptr(z), *ops.strides(z), ops.ptr(bias),
+                softplus, ops.DTYPES[x.dtype], ops.ptr(lengths), ops.ptr(state), B, T, C, N, y.data_ptr(), ops.ptr(final),
+                ops.ptr(ckpt), ops.ptr(ws), nbytes, ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_selective_scan")
         if keep:
             ctx.save_for_backward(x, delta, A, Bm, Cm, D, z, bias, lengths, ckpt)
             ctx.bk_softplus = softplus
-            ctx.bk_state = state is not None
             ctx.set_materialize_grads(False)
         return (y, final) if want_state else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dfinal=None):
-        L = _lib.load()
+        ops.once_only("selective_scan")
         x, delta, A, Bm, Cm, D, z, bias, lengths, ckpt = ctx.saved_tensors
         B, T, C = x.shape
         N = A.shape[1]
-        dev = x.device
-        dy = torch.zeros(B, T, C, dtype=x.dtype, device=dev) if dy is None else ops.inner(dy)
+        dev, dt = x.device, x.dtype
+        dy = torch.zeros(B, T, C, dtype=dt, device=dev) if dy is None else ops.inner(dy)
         dfinal = None if dfinal is None else dfinal.contiguous()
-        dx, dd = torch.empty_like(dy, memory_format=torch.contiguous_format), torch.empty(B, T, C, dtype=x.dtype, device=dev)
-        dz = None if z is None else torch.empty(B, T, C, dtype=x.dtype, device=dev)
-        dB, dC = (torch.empty(B, T, N, dtype=x.dtype, device=dev) for _ in range(2))
+        dx = torch.empty(B, T, C, dtype=dt, device=dev)
+        dd = torch.empty_like(dx)
+        dz = None if z is None else torch.empty_like(dx)
+        dB = torch.empty(B, T, N, dtype=dt, device=dev)
+        dC = torch.empty_like(dB)
         gp = torch.empty(C * N + 2 * C, dtype=torch.float32, device=dev)
-        dh0 = torch.empty(B, C, N, dtype=torch.float32, device=dev) if ctx.bk_state and ctx.needs_input_grad[8] else None
+        dh0 = torch.empty(B, C, N, dtype=torch.float32, device=dev) if ctx.needs_input_grad[8] else None
         if B == 0 or T == 0 or C == 0:       # nothing runs: no position, and the state passes through unchanged
             for t in (gp, dB, dC):
                 t.zero_()
             if dh0 is not None:
                 dh0.zero_() if dfinal is None else dh0.copy_(dfinal)
-        with torch.cuda.device(dev):
-            nbytes = int(L.bkcore_selective_scan_backward_workspace_bytes(B, T, C, N))
-            ws = ops.scratch(nbytes, dev)
+        L = _lib.load_held()
+        nbytes = L.bkcore_selective_scan_backward_workspace_bytes(B, T, C, N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with ops.on_device(dev):
             rc = L.bkcore_selective_scan_backward(
-                ops.ptr(dy), dy.stride(0), dy.stride(1), ops.ptr(dfinal), ops.ptr(x), x.stride(0), x.stride(1),
-                ops.ptr(delta), delta.stride(0), delta.stride(1), ops.ptr(A), ops.ptr(Bm), Bm.stride(0), Bm.stride(1),
-                ops.ptr(Cm), Cm.stride(0), Cm.stride(1), ops.ptr(D), ops.ptr(z), 0 if z is None else z.stride(0),
-                0 if z is None else z.stride(1), ops.ptr(bias), ctx.bk_softplus, ops.DTYPES[x.dtype], ops.ptr(lengths),
-                ops.ptr(ckpt), B, T, C, N, ops.ptr(dx), ops.ptr(dd), ops.ptr(gp), ops.ptr(dB), ops.ptr(dC), ops.ptr(dz),
-                ops.ptr(dh0), ops.ptr(ws), nbytes, ops.stream())
-        _lib.check(rc, "bkcore_selective_scan_backward")
+                dy.data_ptr(), *ops.strides(dy), ops.ptr(dfinal), x.data_ptr(), *ops.strides(x), delta.data_ptr(),
+                *ops.strides(delta), A.data_ptr(), Bm.data_ptr(), *ops.strides(Bm), Cm.data_ptr(), *ops.strides(Cm),
+                ops.ptr(D), ops.ptr(z), *ops.strides(z), ops.ptr(bias), ctx.bk_softplus, ops.DTYPES[dt], ops.ptr(lengths),
+                ckpt.data_ptr(), B, T, C, N, dx.data_ptr(), dd.data_ptr(), gp.data_ptr(), dB.data_ptr(), dC.data_ptr(),
+                ops.ptr(dz), ops.ptr(dh0), ws.data_ptr(), nbytes, ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_selective_scan_backward")
         grads = (dx, dd, gp[:C * N].view(C, N), dB, dC, gp[C * N:C * N + C], dz, gp[C * N + C:], dh0)
         return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad)) + (None,) * 4
 
@@ -254,7 +262,6 @@ def selective_scan_step(x: torch.Tensor, state: torch.Tensor, delta: torch.Tenso
     what = "selective_scan_step"
     if x.dim() != 2:
         raise ValueError(f"bkcore: {what}: x is (B, C), got {tuple(x.shape)}")
-    L = _lib.load()
     b, c = x.shape
     ops.need_device(x, delta, B, C, z, state)
     code = ops.need_dtype(what, x, delta, B, C, z)
@@ -268,12 +275,14 @@ def selective_scan_step(x: torch.Tensor, state: torch.Tensor, delta: torch.Tenso
         raise ValueError(f"bkcore: {what}: state must be contiguous and 16-byte aligned")
     if A.data_ptr() % 16:
         A = A.clone()
-    x, delta, B, C, z = (ops.inner(t) for t in (x, delta, B, C, z))
-    y = torch.empty(b, c, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = L.bkcore_selective_scan_step(ops.ptr(x), x.stride(0), ops.ptr(state), ops.ptr(delta), delta.stride(0),
-                                          ops.ptr(A), ops.ptr(B), B.stride(0), ops.ptr(C), C.stride(0), ops.ptr(D),
-                                          ops.ptr(z), 0 if z is None else z.stride(0), ops.ptr(delta_bias),
-                                          int(bool(delta_softplus)), code, b, c, n, ops.ptr(y), ops.stream())
-    _lib.check(rc, "bkcore_selective_scan_step")
+    x, delta, B, C, z = ops.inner(x), ops.inner(delta), ops.inner(B), ops.inner(C), ops.inner(z)
+    dev = x.device
+    y = torch.empty(b, c, dtype=x.dtype, device=dev)
+    with ops.on_device(dev):
+        rc = _lib.load_held().bkcore_selective_scan_step(
+            x.data_ptr(), x.stride(0), state.data_ptr(), delta.data_ptr(), delta.stride(0), A.data_ptr(), B.data_ptr(),
+            B.stride(0), C.data_ptr(), C.stride(0), ops.ptr(D), ops.ptr(z), 0 if z is None else z.stride(0),
+            ops.ptr(delta_bias), int(bool(delta_softplus)), code, b, c, n, y.data_ptr(), ops.stream(dev.index))
+    if rc:
+        _lib.check(rc, "bkcore_selective_scan_step")
     return y

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int 
 }
 
 // One workgroup: 32 channel vectors x 8 stretches of 32 positions of one sequence.  part: one row of (K + 1) C floats
-// per (sequence, workgroup along time): K rows of the weights' sums, then the bias'.
+// per (sequence, workgroup along time): the weights' sums (C, K), then the bias'.
 template <typename T, int K, int V>
 __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(ConvArgs a, int nblk, int cblk) {
   __shared__ float join[BWD_SEGS][BWD_CH][V + 1];
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
         float s = 0.0f;
 #pragma unroll
         for (int q = 0; q < BWD_SEGS; ++q) s += join[q][j / V][j % V];
-        out[(long)k * a.C + col] = s;
+        out[k < K ? (long)col * K + k : (long)K * a.C + col] = s;
       }
     }
   }
