@@ -13,6 +13,7 @@ using namespace bk;
 
 constexpr int FWD_TL = 16;  // positions a thread walks forward: 3 of 19 reads are repeated
 constexpr int BWD_TL = 32;  // ... and backward
+constexpr int BWD_UNDER = 5; // positions loaded ahead of their use: 35 = 32 + K - 1 of four taps in seven blocks
 constexpr int BWD_SEGS = 8; // stretches of one workgroup, joined before the partial sums are written
 constexpr int BWD_CH = 32;  // channel vectors of one workgroup
 
@@ -67,29 +68,36 @@ __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int 
   const long r = id / nvec;
   const int seg = (int)(r % nseg), b = (int)(r / nseg);
   const int len = row_length(a.lengths, b, a.L);
-  float w[K][V], bias[V], h[K][V];
-  load_taps<T, K, V>(a, c, w, bias);
-  const long t0 = (long)seg * FWD_TL, t1 = t0 + FWD_TL < a.L ? t0 + FWD_TL : a.L;
+  const int t0 = seg * FWD_TL, t1 = t0 + FWD_TL < a.L ? t0 + FWD_TL : a.L;
+  if (t0 < a.L) {
+    const T *x = (const T *)a.x + b * a.xb + c;
+    RawVec<T, V> raw[FWD_TL];  // all of the stretch is under way before its first position is worked on
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) input_at<T, K, V>(a, b, t0 - (K - 1) + k, len, c, h[k]);
-  T *y = (T *)a.y + ((long)b * a.L) * a.C + c;
-#pragma unroll 4
-  for (long t = t0; t < t1; ++t) {
-    input_at<T, K, V>(a, b, t, len, c, h[K - 1]);
-    float o[V];
+    for (int j = 0; j < FWD_TL; ++j) raw[j].load(x + (long)(t0 + j < a.L ? t0 + j : a.L - 1) * a.xt);
+    float w[K][V], bias[V], h[K][V];
+    load_taps<T, K, V>(a, c, w, bias);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float s = bias[i];
+    for (int k = 0; k < K - 1; ++k) input_at<T, K, V>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+    T *y = (T *)a.y + ((long)b * a.L) * a.C + c;
 #pragma unroll
-      for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
-      if (a.silu) s = s * sigmoid(s);
-      o[i] = t < len ? s : 0.0f;
+    for (int j = 0; j < FWD_TL; ++j) {
+      const int t = t0 + j;
+      raw[j].get(t < len, h[K - 1]);
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float s = bias[i];
+#pragma unroll
+        for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
+        if (a.silu) s = s * sigmoid(s);
+        o[i] = t < len ? s : 0.0f;
+      }
+      if (t < t1) store_vec<T, V>(y + (long)t * a.C, o);
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[k][i] = h[k + 1][i];
     }
-    store_vec<T, V>(y + t * a.C, o);
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[k][i] = h[k + 1][i];
   }
   if (a.final_state && seg == 0) {  // the last K - 1 inputs, the carried ones among them for a short sequence
 #pragma unroll
@@ -134,11 +142,23 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
     const T *dy = (const T *)a.dy + b * a.dyb + c;
     T *dx = (T *)a.dx + (long)b * a.L * a.C + c;
     // dx of position t - K + 1 is complete once g_t is known; the first stretch also gives the carried state's gradient
-    for (long t = t0; t < t1 + K - 1; ++t) {
+    const T *x = (const T *)a.x + b * a.xb + c;
+    for (long tb0 = t0; tb0 < t1 + K - 1; tb0 += BWD_UNDER) {
+    RawVec<T, V> rx[BWD_UNDER], rg[BWD_UNDER];  // so many positions are under way at once
+#pragma unroll
+    for (int j = 0; j < BWD_UNDER; ++j) {
+      const long t = tb0 + j < a.L ? tb0 + j : a.L - 1;
+      rx[j].load(x + t * a.xt);
+      rg[j].load(dy + t * a.dyt);
+    }
+#pragma unroll
+    for (int j = 0; j < BWD_UNDER; ++j) {
+      const long t = tb0 + j;
+      if (t >= t1 + K - 1) break;
       if (t < len) {
-        input_at<T, K, V>(a, b, t, len, c, h[K - 1]);
         float d[V];
-        load_vec<T, V>(dy + t * a.dyt, d);
+        rx[j].get(true, h[K - 1]);
+        rg[j].get(true, d);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if (a.silu) {
@@ -188,6 +208,7 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
           h[k][i] = h[k + 1][i];
           g[k][i] = g[k + 1][i];
         }
+    }
     }
   }
   if (!a.part) return;

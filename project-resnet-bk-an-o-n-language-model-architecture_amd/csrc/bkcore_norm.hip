@@ -31,21 +31,25 @@ __device__ __forceinline__ float row_sum(float x, float *lds, int slot) {
 
 // Element i of thread t's E elements, V at a time: column ((i / V) * TPR + t) * V + i % V.
 template <typename T, int TPR, int E, int V>
-__device__ __forceinline__ void load_row(const T *__restrict__ p, int t, int D, float (&v)[E]) {
+struct Row {
+  RawVec<T, V> r[E / V];
+  __device__ __forceinline__ void load(const T *__restrict__ p, int t, int D) {
 #pragma unroll
-  for (int c = 0; c < E / V; ++c) {
-    const int col = (c * TPR + t) * V;
-    float w[V];
-    if (col < D) {
-      load_vec<T, V>(p + col, w);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = 0.0f;
+    for (int c = 0; c < E / V; ++c) {
+      const int col = (c * TPR + t) * V;
+      r[c].load(p + (col < D ? col : 0));
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[c * V + i] = w[i];
   }
-}
+  __device__ __forceinline__ void get(int t, int D, float (&v)[E]) const {
+#pragma unroll
+    for (int c = 0; c < E / V; ++c) {
+      float w[V];
+      r[c].get((c * TPR + t) * V < D, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[c * V + i] = w[i];
+    }
+  }
+};
 
 template <typename T, int TPR, int E, int V>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_kernel(
@@ -57,7 +61,9 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_kernel(
   const long row = (long)blockIdx.x * RPB + (TPR == 64 ? threadIdx.x >> 6 : 0);
   if (row >= rows) return;  // uniform in the wave (TPR 64) or in the workgroup
   float v[E];
-  load_row<T, TPR, E, V>(x + row * ldx, t, D, v);
+  Row<T, TPR, E, V> raw;
+  raw.load(x + row * ldx, t, D);
+  raw.get(t, D, v);
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < E; ++i) s += v[i];
@@ -114,11 +120,23 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_backward_
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
   int slot = 0;
-  for (long row = (long)blockIdx.x * RPB + sub; row < rows; row += (long)gridDim.x * RPB) {
-    const float mean = stats[row], rstd = stats[rows + row];
+  Row<T, TPR, E, V> rg, rx;  // the next row is under way while this one is worked on
+  float rmean, rrstd;
+  auto fetch = [&](long row) {
+    rg.load(dy + row * lddy, t, D);
+    rx.load(x + row * ldx, t, D);
+    rmean = stats[row];
+    rrstd = stats[rows + row];
+  };
+  const long first = (long)blockIdx.x * RPB + sub;
+  if (first < rows) fetch(first);
+  for (long row = first; row < rows; row += (long)gridDim.x * RPB) {
     float g[E], h[E];
-    load_row<T, TPR, E, V>(dy + row * lddy, t, D, g);
-    load_row<T, TPR, E, V>(x + row * ldx, t, D, h);
+    rg.get(t, D, g);
+    rx.get(t, D, h);
+    const float mean = rmean, rstd = rrstd;
+    const long next = row + (long)gridDim.x * RPB;
+    if (next < rows) fetch(next);
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
     for (int c = 0; c < E / V; ++c) {

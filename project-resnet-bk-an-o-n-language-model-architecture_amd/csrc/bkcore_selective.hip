@@ -17,7 +17,8 @@
 // every chunk's end state from a zero start with the sum of its d (the chunk's decay is exp(A sum d)), the next one folds
 // those in front of its chunk and runs the chunk from there.
 // The backward needs h at every position: the forward keeps it at every 16th (e.g. 4 bytes a position and channel for 16
-// states), and a tile of 16 positions recomputes the rest, transitions included, into registers.
+// states), and a tile of 16 positions recomputes the rest into registers (the transitions twice: kept
+// beside the states they would not fit).
 // The sums over channels (dB, dC) are folded across the wave by lane exchanges, across the workgroup's waves in LDS and
 // across workgroups by a second launch; every order is fixed, results do not change from run to run.
 // States, statistics and sums are float32 whatever the operands' type.
@@ -29,7 +30,8 @@ using namespace bk;
 constexpr int TILE = 16;       // positions of a tile; a checkpoint in front of each
 constexpr int WAVES = 4;       // waves of a workgroup
 constexpr int THREADS = 64 * WAVES;
-constexpr int MAX_CHUNKS = 32; // a chunk folds all chunks in front of it by itself
+constexpr int MAX_CHUNKS = 64; // a chunk folds all chunks in front of it by itself: 512 channels x 8191 positions 70 us
+                               // with at most 32, 56 with 64, 64 with 128
 
 struct ScanArgs {
   const void *x, *delta, *z, *Bm, *Cm, *dy;
@@ -58,9 +60,13 @@ __device__ __forceinline__ float sum_states(float v) {
 }
 
 // The value of lane Q of each quad.
+// (The empty asm keeps the move a move: folded into its eight users it would make each of them a DPP instruction at 4.3
+// cycles instead of 2.4.)
 template <int Q>
 __device__ __forceinline__ float quad_get(float v) {
-  return dpp_mov<Q * 0x55>(v);
+  float r = dpp_mov<Q * 0x55>(v);
+  asm("" : "+v"(r));
+  return r;
 }
 
 // log(1 + e^p): with u = 1 + e^p the correction e^p / (u - 1) keeps the relative accuracy where e^p is small; from 20 on
@@ -88,28 +94,51 @@ struct Place {
   }
 };
 
-// B_t, C_t of a tile on their way to LDS: N padded to NP = 4 LPC states with zeros.
+// B_t, C_t of a tile on their way to LDS: N padded to NP = 4 LPC states with zeros.  Loads are unconditional (from the
+// nearest valid place) and stay in the operands' type until they are used: a load under a condition, or converted where it
+// is issued, would be waited for at once.
 template <typename T, int LPC>
 struct StateRows {
   static constexpr int NP = 4 * LPC;
   static constexpr int PER = TILE * NP / THREADS;
-  float b[PER], c[PER];
-  __device__ __forceinline__ void load(const ScanArgs &a, int bi, long t0, int len, bool want_b, bool want_c) {
+  T b[PER], c[PER];
+  __device__ __forceinline__ void load(const ScanArgs &a, int bi, long t0, long stop, bool want_b, bool want_c) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int i = threadIdx.x + k * THREADS, n = i % NP;
-      const long t = t0 + i / NP;
-      const bool in = t < len && n < a.N;
-      b[k] = want_b && in ? at<T>(a.Bm, bi * a.Bb + t * a.Bt + n) : 0.0f;
-      c[k] = want_c && in ? at<T>(a.Cm, bi * a.Cb + t * a.Ct + n) : 0.0f;
+      const unsigned t = min((unsigned)(i / NP), (unsigned)(stop - 1 - t0 < TILE ? stop - 1 - t0 : TILE));
+      const unsigned nn = n < a.N ? n : 0;
+      if (want_b) b[k] = ((const T *)a.Bm + bi * a.Bb + t0 * a.Bt)[t * (unsigned)a.Bt + nn];
+      if (want_c) c[k] = ((const T *)a.Cm + bi * a.Cb + t0 * a.Ct)[t * (unsigned)a.Ct + nn];
     }
   }
-  __device__ __forceinline__ void store(float *sb, float *sc) const {
+  __device__ __forceinline__ void store(const ScanArgs &a, long t0, long stop, float *sb, float *sc) const {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int i = threadIdx.x + k * THREADS;
-      sb[i] = b[k];
-      sc[i] = c[k];
+      const bool in = t0 + i / NP < stop && i % NP < a.N;
+      if (sb) sb[i] = in ? (float)b[k] : 0.0f;
+      if (sc) sc[i] = in ? (float)c[k] : 0.0f;
+    }
+  }
+};
+
+// Four positions of a lane's quad (t0 + 4 i + q) of a (B, L, C) operand, in its own type.  The address is a uniform
+// 64-bit base of the tile and a 32-bit offset inside it (the host keeps 16 strides below 2^31), which saves the register
+// pairs that full addresses would take.
+template <typename T>
+struct Column {
+  const T *p;
+  long step;
+  T v[4];
+  __device__ __forceinline__ Column(const void *base, long off, long step_) : p((const T *)base + off), step(step_) {}
+  __device__ __forceinline__ void load(long t0, int q, int c, long stop) {
+    const T *tile = p + t0 * step;
+    const unsigned most = (unsigned)(stop - 1 - t0 < TILE ? stop - 1 - t0 : TILE), st = (unsigned)step;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned t = min((unsigned)(4 * i + q), most);
+      v[i] = tile[t * st + (unsigned)c];
     }
   }
 };
@@ -135,7 +164,7 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
   }
   const float skip = live && a.D ? a.D[c] : 0.0f, bias = live && a.bias ? a.bias[c] : 0.0f;
   if (!AGG && live) {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < s; ++j) {
       const long at0 = ((long)j * a.B + b) * a.C + c;
       const float sd = a.aggd[at0];
@@ -144,18 +173,15 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
       for (int n = 0; n < 4; ++n) h[n] = fmaf(exp2_fast(A2[n] * sd), h[n], e[n]);
     }
   }
-  float xr[4], dr[4], zr[4], sum_d = 0.0f;
+  float sum_d = 0.0f;
+  const int cc = live ? c : a.C - 1;
+  Column<T> xr(a.x, b * a.xb, a.xt), dr(a.delta, b * a.db, a.dt), zr(a.z, b * a.zb, a.zt);
   StateRows<T, LPC> rows;
   auto prefetch = [&](long t0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long t = t0 + 4 * i + q;
-      const bool in = live && t < stop;
-      xr[i] = in ? at<T>(a.x, b * a.xb + t * a.xt + c) : 0.0f;
-      dr[i] = in ? at<T>(a.delta, b * a.db + t * a.dt + c) + bias : 0.0f;
-      if (!AGG) zr[i] = in && a.z ? at<T>(a.z, b * a.zb + t * a.zt + c) : 0.0f;
-    }
-    rows.load(a, b, t0, (int)stop, true, !AGG);
+    xr.load(t0, q, cc, stop);
+    dr.load(t0, q, cc, stop);
+    if (!AGG && a.z) zr.load(t0, q, cc, stop);
+    rows.load(a, b, t0, stop, true, !AGG);
   };
   if (begin < stop) prefetch(begin);
   int buf = 0;
@@ -164,14 +190,15 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool in = live && t0 + 4 * i + q < stop;
-      xv[i] = xr[i];
-      if (!AGG) zv[i] = zr[i];
-      dv[i] = in ? (a.softplus ? softplus(dr[i]) : dr[i]) : 0.0f;
+      xv[i] = in ? (float)xr.v[i] : 0.0f;
+      if (!AGG) zv[i] = in && a.z ? (float)zr.v[i] : 0.0f;
+      const float p = (float)dr.v[i] + bias;
+      dv[i] = in ? (a.softplus ? softplus(p) : p) : 0.0f;
       ux[i] = dv[i] * xv[i];
       if (AGG) sum_d += dv[i];
       yv[i] = 0.0f;
     }
-    rows.store(sB[buf], sC[buf]);
+    rows.store(a, t0, stop, sB[buf], AGG ? nullptr : sC[buf]);
     __syncthreads();
     if (t0 + TILE < stop) prefetch(t0 + TILE);
     if (!AGG && a.ckpt && live) {
@@ -179,7 +206,7 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
 #pragma unroll
       for (int n = 0; n < 4; ++n) k[n] = h[n];
       const long tile = t0 / TILE, ntiles = (a.L + TILE - 1) / TILE;
-      *reinterpret_cast<f32x4 *>(a.ckpt + ((b * ntiles + tile) * a.C + c) * NP + sub * 4) = k;
+      *reinterpret_cast<f32x4 *>(a.ckpt + (b * ntiles + tile) * a.C * NP + (unsigned)(c * NP + sub * 4)) = k;
     }
 #define BK_STEP(i, Q)                                                                            \
   do {                                                                                           \
@@ -204,13 +231,14 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
     }
 #undef BK_STEP
     if (!AGG && live && sub < 4) {
+      T *out = (T *)a.y + ((long)b * a.L + t0) * a.C;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long t = t0 + 4 * i + q;
         if (t < end) {
           float y = fmaf(skip, xv[i], yv[i]);
           if (a.z) y *= zv[i] * sigmoid(zv[i]);
-          ((T *)a.y)[((long)b * a.L + t) * a.C + c] = (T)(t < stop ? y : 0.0f);
+          out[(unsigned)((4 * i + q) * a.C + c)] = (T)(t < stop ? y : 0.0f);
         }
       }
     }
@@ -243,7 +271,7 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
 template <typename T, int LPC>
 __global__ __launch_bounds__(THREADS) void bk_scan_adjoint_agg_kernel(ScanArgs a) {
   constexpr int NP = 4 * LPC, CPW = 64 / LPC;
-  __shared__ float sB[2][TILE * NP], sC[2][TILE * NP];
+  __shared__ float sC[2][TILE * NP];
   const Place at_(a);
   const int b = at_.b, s = at_.s + 1, lane = threadIdx.x & 63, sub = lane % LPC, q = lane & 3;
   const int c = (at_.ct * WAVES + (threadIdx.x >> 6)) * CPW + lane / LPC;
@@ -259,18 +287,15 @@ __global__ __launch_bounds__(THREADS) void bk_scan_adjoint_agg_kernel(ScanArgs a
     carry[n] = 0.0f;
   }
   const float bias = live && a.bias ? a.bias[c] : 0.0f;
-  float dr[4], zr[4], gr[4], sum_d = 0.0f;
+  float sum_d = 0.0f;
+  const int cc = live ? c : a.C - 1;
+  Column<T> dr(a.delta, b * a.db, a.dt), gr(a.dy, b * a.yb, a.yt), zr(a.z, b * a.zb, a.zt);
   StateRows<T, LPC> rows;
   auto prefetch = [&](long t0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long t = t0 + 4 * i + q;
-      const bool in = live && t < stop;
-      dr[i] = in ? at<T>(a.delta, b * a.db + t * a.dt + c) + bias : 0.0f;
-      gr[i] = in ? at<T>(a.dy, b * a.yb + t * a.yt + c) : 0.0f;
-      zr[i] = in && a.z ? at<T>(a.z, b * a.zb + t * a.zt + c) : 0.0f;
-    }
-    rows.load(a, b, t0, (int)stop, false, true);
+    dr.load(t0, q, cc, stop);
+    gr.load(t0, q, cc, stop);
+    if (a.z) zr.load(t0, q, cc, stop);
+    rows.load(a, b, t0, stop, false, true);
   };
   const long last = begin + (stop - begin + TILE - 1) / TILE * TILE - TILE;
   if (begin < stop) prefetch(last);
@@ -280,11 +305,12 @@ __global__ __launch_bounds__(THREADS) void bk_scan_adjoint_agg_kernel(ScanArgs a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool in = live && t0 + 4 * i + q < stop;
-      dv[i] = in ? (a.softplus ? softplus(dr[i]) : dr[i]) : 0.0f;
-      uv[i] = a.z ? gr[i] * (zr[i] * sigmoid(zr[i])) : gr[i];
+      const float p = (float)dr.v[i] + bias, g = in ? (float)gr.v[i] : 0.0f, z = in && a.z ? (float)zr.v[i] : 0.0f;
+      dv[i] = in ? (a.softplus ? softplus(p) : p) : 0.0f;
+      uv[i] = a.z ? g * (z * sigmoid(z)) : g;
       sum_d += dv[i];
     }
-    rows.store(sB[buf], sC[buf]);
+    rows.store(a, t0, stop, nullptr, sC[buf]);
     __syncthreads();
     if (t0 - TILE >= begin) prefetch(t0 - TILE);
 #define BK_STEP(i, Q)                                                                            \
@@ -340,7 +366,7 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
   }
   const float skip = live && a.D ? a.D[c] : 0.0f, bias = live && a.bias ? a.bias[c] : 0.0f;
   if (live) {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = a.S - 1; j > s; --j) {
       const long at0 = ((long)j * a.B + b) * a.C + c;
       const float sd = a.aggd[at0];
@@ -350,43 +376,39 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
     }
   }
   const long ntiles = (a.L + TILE - 1) / TILE;
-  float xr[4], dr[4], zr[4], gr[4];
-  f32x4 hr = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int cc = live ? c : a.C - 1;
+  Column<T> xr(a.x, b * a.xb, a.xt), dr(a.delta, b * a.db, a.dt), gr(a.dy, b * a.yb, a.yt), zr(a.z, b * a.zb, a.zt);
+  f32x4 hr;
   StateRows<T, LPC> rows;
   auto prefetch = [&](long t0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long t = t0 + 4 * i + q;
-      const bool in = live && t < stop;
-      xr[i] = in ? at<T>(a.x, b * a.xb + t * a.xt + c) : 0.0f;
-      dr[i] = in ? at<T>(a.delta, b * a.db + t * a.dt + c) + bias : 0.0f;
-      gr[i] = in ? at<T>(a.dy, b * a.yb + t * a.yt + c) : 0.0f;
-      zr[i] = in && a.z ? at<T>(a.z, b * a.zb + t * a.zt + c) : 0.0f;
-    }
-    if (live) hr = *reinterpret_cast<const f32x4 *>(a.ckpt + ((b * ntiles + t0 / TILE) * a.C + c) * NP + sub * 4);
-    rows.load(a, b, t0, (int)stop, true, true);
+    xr.load(t0, q, cc, stop);
+    dr.load(t0, q, cc, stop);
+    gr.load(t0, q, cc, stop);
+    if (a.z) zr.load(t0, q, cc, stop);
+    hr = *reinterpret_cast<const f32x4 *>(a.ckpt + (b * ntiles + t0 / TILE) * a.C * NP + (unsigned)(cc * NP + sub * 4));
+    rows.load(a, b, t0, stop, true, true);
   };
   const long last = begin + (stop - begin + TILE - 1) / TILE * TILE - TILE;
   if (begin < stop) prefetch(last);
   int buf = 0;
   for (long t0 = last; begin < stop && t0 >= begin; t0 -= TILE, buf ^= 1) {
     float xv[4], dv[4], pv[4], uv[4], gv[4], ux[4], yv[4], gb[4], sa[4], zv[4];
-    float h0[4], h[TILE][4], e[TILE][4];
+    float h0[4], h[TILE][4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) h0[n] = hr[n];
+    for (int n = 0; n < 4; ++n) h0[n] = live ? hr[n] : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool in = live && t0 + 4 * i + q < stop;
-      xv[i] = xr[i];
-      zv[i] = zr[i];
-      gv[i] = gr[i];
-      pv[i] = dr[i];
-      dv[i] = in ? (a.softplus ? softplus(dr[i]) : dr[i]) : 0.0f;
+      xv[i] = in ? (float)xr.v[i] : 0.0f;
+      zv[i] = in && a.z ? (float)zr.v[i] : 0.0f;
+      gv[i] = in ? (float)gr.v[i] : 0.0f;
+      pv[i] = (float)dr.v[i] + bias;
+      dv[i] = in ? (a.softplus ? softplus(pv[i]) : pv[i]) : 0.0f;
       ux[i] = dv[i] * xv[i];
       uv[i] = a.z ? gv[i] * (zv[i] * sigmoid(zv[i])) : gv[i];
       yv[i] = gb[i] = sa[i] = 0.0f;
     }
-    rows.store(sB[buf], sC[buf]);
+    rows.store(a, t0, stop, sB[buf], sC[buf]);
     __syncthreads();
     if (t0 - TILE >= begin) prefetch(t0 - TILE);
 #define BK_STEP(i, Q)                                                                            \
@@ -397,8 +419,7 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
     float y = 0.0f;                                                                              \
     const f32x4 Cv = *reinterpret_cast<const f32x4 *>(&sC[buf][t_ * NP + sub * 4]);              \
     _Pragma("unroll") for (int n = 0; n < 4; ++n) {                                              \
-      e[t_][n] = exp2_fast(d * A2[n]);                                                           \
-      h[t_][n] = fmaf(e[t_][n], t_ ? h[t_ ? t_ - 1 : 0][n] : h0[n], u * Bv[n]);                  \
+      h[t_][n] = fmaf(exp2_fast(d * A2[n]), t_ ? h[t_ ? t_ - 1 : 0][n] : h0[n], u * Bv[n]);      \
       y = fmaf(h[t_][n], Cv[n], y);                                                              \
     }                                                                                            \
     if (a.z) {                                                                                   \
@@ -406,13 +427,21 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
       if (q == Q) yv[i] = y;                                                                     \
     }                                                                                            \
   } while (0)
-#define BK_STEPS(i) BK_STEP(i, 0); BK_STEP(i, 1); BK_STEP(i, 2); BK_STEP(i, 3)
+// The barriers keep the scheduler from raising the LDS reads of all sixteen positions to the top, which spills.
+#define BK_STEPS(i) BK_STEP(i, 0); BK_STEP(i, 1); BK_STEP(i, 2); BK_STEP(i, 3); __builtin_amdgcn_sched_barrier(0)
     BK_STEPS(0);
     BK_STEPS(1);
     BK_STEPS(2);
     BK_STEPS(3);
 #undef BK_STEPS
 #undef BK_STEP
+    // The transitions are formed again in the way back: the compiler would keep the first ones (64 registers) and spill.
+    float A2r[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      A2r[n] = A2[n];
+      asm volatile("" : "+v"(A2r[n]));
+    }
     float pair[4];  // (position, dB or dC) sums of two positions, waiting to be written together
 #define BK_STEP(i, Q)                                                                            \
   do {                                                                                           \
@@ -426,7 +455,7 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
       vC[n] = u * h[t_][n];                                                                      \
       vB[n] = g * ud;                                                                            \
       gB = fmaf(g, Bv[n], gB);                                                                   \
-      carry[n] = g * e[t_][n];                                                                   \
+      carry[n] = g * exp2_fast(d * A2r[n]);                                                      \
       const float eh = carry[n] * (t_ ? h[t_ ? t_ - 1 : 0][n] : h0[n]);                          \
       sA = fmaf(eh, A2[n], sA);                                                                  \
       dA[n] = fmaf(eh, d, dA[n]);                                                                \
@@ -453,7 +482,11 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
       }                                                                                          \
     }                                                                                            \
   } while (0)
-#define BK_STEPS(i) BK_STEP(i, 3); BK_STEP(i, 2); BK_STEP(i, 1); BK_STEP(i, 0)
+// The sums over positions are pinned to their place: sunk behind the tile they would keep all 64 of their terms alive.
+#define BK_STEPS(i)                                                                              \
+  BK_STEP(i, 3); BK_STEP(i, 2); BK_STEP(i, 1); BK_STEP(i, 0);                                    \
+  asm volatile("" : "+v"(dA[0]), "+v"(dA[1]), "+v"(dA[2]), "+v"(dA[3]));                        \
+  __builtin_amdgcn_sched_barrier(0)
     BK_STEPS(3);
     BK_STEPS(2);
     BK_STEPS(1);
@@ -461,21 +494,23 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
 #undef BK_STEPS
 #undef BK_STEP
     if (live && sub < 4) {
+      const long tile = ((long)b * a.L + t0) * a.C;
+      T *dx = (T *)a.dx + tile, *ddl = (T *)a.ddelta + tile, *dzo = a.z ? (T *)a.dz + tile : nullptr;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long t = t0 + 4 * i + q;
         if (t < end) {
           const bool in = t < stop;
-          const long o = ((long)b * a.L + t) * a.C + c;
+          const unsigned o = (unsigned)((4 * i + q) * a.C + c);
           const float dxo = fmaf(dv[i], gb[i], skip * uv[i]);
           float dd = fmaf(xv[i], gb[i], sa[i] * (1.0f / LOG2E));
           if (a.softplus) dd *= pv[i] > 20.0f ? 1.0f : sigmoid(pv[i]);
-          ((T *)a.dx)[o] = (T)(in ? dxo : 0.0f);
-          ((T *)a.ddelta)[o] = (T)(in ? dd : 0.0f);
+          dx[o] = (T)(in ? dxo : 0.0f);
+          ddl[o] = (T)(in ? dd : 0.0f);
           if (a.z) {
             const float sg = sigmoid(zv[i]);
             const float dz = gv[i] * fmaf(skip, xv[i], yv[i]) * (sg * fmaf(zv[i], 1.0f - sg, 1.0f));
-            ((T *)a.dz)[o] = (T)(in ? dz : 0.0f);
+            dzo[o] = (T)(in ? dz : 0.0f);
           }
           if (in) {
             dD = fmaf(uv[i], xv[i], dD);
@@ -596,7 +631,8 @@ __global__ __launch_bounds__(256) void bk_scan_step_kernel(ScanArgs a, float *__
 inline int lanes_per_channel(int64_t N) { return N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 // Chunks of the time axis: one while the channels alone give every SIMD a wave (cutting adds a pass over the inputs),
-// else enough for two waves a SIMD, of at least four tiles each.
+// else enough for four waves a SIMD, of at least four tiles each (4 x 2048 positions x 1024 channels, both launches of the
+// forward: 97 us at two waves, 86 at four, 95 at six).
 struct Plan {
   int lpc, nct, S, chunk;
 };
@@ -608,7 +644,7 @@ inline Plan plan(int64_t B, int64_t L, int64_t C, int64_t N) {
   const int64_t waves = B * p.nct * WAVES;
   int64_t S = 1;
   if (waves < 1024) {
-    S = 2048 / (waves > 0 ? waves : 1);
+    S = 4096 / (waves > 0 ? waves : 1);
     const int64_t most = L / (4 * TILE);
     if (S > most) S = most;
     if (S > MAX_CHUNKS) S = MAX_CHUNKS;
@@ -629,6 +665,9 @@ int check(int dtype, int64_t B, int64_t L, int64_t C, int64_t N) {
   if (B > (1 << 24) || L > (1 << 30) || C > (1 << 24)) return BKCORE_EINVAL;
   return BKCORE_OK;
 }
+
+// 16 positions of an operand within 32-bit offsets
+inline bool near(int64_t time_stride) { return time_stride >= 0 && time_stride < (1LL << 26); }
 
 inline size_t agg_floats(const Plan &p, int64_t B, int64_t C) {
   return p.S > 1 ? (size_t)p.S * B * C * (4 * p.lpc + 1) : 0;
@@ -666,6 +705,7 @@ extern "C" int bkcore_selective_scan(const void *x, int64_t x_batch, int64_t x_t
   if (rc) return rc;
   if (B == 0 || C == 0 || L == 0) return BKCORE_OK;
   if (!x || !delta || !A || !Bm || !Cm || !y) return BKCORE_EINVAL;
+  if (!near(x_time) || !near(delta_time) || !near(B_time) || !near(C_time) || (z && !near(z_time))) return BKCORE_EINVAL;
   const Plan p = plan(B, L, C, N);
   if (p.S > 1 && (!workspace || workspace_bytes < bkcore_selective_scan_workspace_bytes(B, L, C, N)))
     return BKCORE_EWORKSPACE;
@@ -709,6 +749,8 @@ extern "C" int bkcore_selective_scan_backward(
   if (B == 0 || C == 0 || L == 0) return BKCORE_OK;
   if (!dy || !x || !delta || !A || !Bm || !Cm || !checkpoints || !dx || !grad_delta || !grad_params || !dB || !dC ||
       (z && !dz))
+    return BKCORE_EINVAL;
+  if (!near(x_time) || !near(delta_time) || !near(B_time) || !near(C_time) || !near(dy_time) || (z && !near(z_time)))
     return BKCORE_EINVAL;
   if (!workspace || workspace_bytes < bkcore_selective_scan_backward_workspace_bytes(B, L, C, N))
     return BKCORE_EWORKSPACE;

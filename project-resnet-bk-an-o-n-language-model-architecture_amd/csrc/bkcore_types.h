@@ -53,6 +53,25 @@ __device__ __forceinline__ void load_vec(const T *__restrict__ p, float (&v)[V])
   }
 }
 
+// The same in two steps, so that several loads are under way before the first is waited for: a load converted where it
+// is issued, or issued under a condition, is waited for at once.
+template <typename T, int V>
+struct RawVec {
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  vec_t w;
+  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *reinterpret_cast<const vec_t *>(p); }
+  __device__ __forceinline__ void get(bool in, float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = in ? (float)w[i] : 0.0f;
+  }
+};
+template <typename T>
+struct RawVec<T, 1> {
+  T w;
+  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *p; }
+  __device__ __forceinline__ void get(bool in, float (&v)[1]) const { v[0] = in ? (float)w : 0.0f; }
+};
+
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T *__restrict__ p, const float (&v)[V]) {
   if constexpr (V == 1) {
