@@ -13,7 +13,7 @@ using namespace bk;
 
 constexpr int FWD_TL = 16;  // positions a thread walks forward: 3 of 19 reads are repeated
 constexpr int BWD_TL = 32;  // ... and backward
-constexpr int BWD_UNDER = 5; // positions loaded ahead of their use: 35 = 32 + K - 1 of four taps in seven blocks
+constexpr int BWD_UNDER = 5; // positions of a block; the next block is under way while one is worked on
 constexpr int BWD_SEGS = 8; // stretches of one workgroup, joined before the partial sums are written
 constexpr int BWD_CH = 32;  // channel vectors of one workgroup
 
@@ -23,7 +23,7 @@ struct ConvArgs {
   float *part;
   const int *lengths;
   long xb, xt, dyb, dyt;  // strides of x and dy in elements
-  int B, L, C, param_f32, silu;
+  int B, L, C, param_f32, param_vec, silu;
 };
 
 __device__ __forceinline__ int row_length(const int *lengths, int b, int L) {
@@ -45,17 +45,26 @@ __device__ __forceinline__ void input_at(const ConvArgs &a, int b, long t, int l
   }
 }
 
+// The taps of V channels are V K neighbouring values; in float32 and aligned they come as 16-byte loads.
 template <typename T, int K, int V>
 __device__ __forceinline__ void load_taps(const ConvArgs &a, int c, float (&w)[K][V], float (&bias)[V]) {
+  float flat[V * K];
+  if (V > 1 && a.param_vec) {
+    const f32x4 *p = reinterpret_cast<const f32x4 *>((const float *)a.w + (long)c * K);
+#pragma unroll
+    for (int j = 0; j < V * K / 4; ++j) {
+      const f32x4 v = p[j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) flat[4 * j + i] = v[i];
+    }
+  } else {
+    load_param<T, V * K>(a.w, a.param_f32, (long)c * K, flat);
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float t[1];
-      load_param<T, 1>(a.w, a.param_f32, (long)(c + i) * K + k, t);
-      w[k][i] = t[0];
-    }
     bias[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][i] = flat[i * K + k];
   }
   if (a.bias) load_param<T, V>(a.bias, a.param_f32, c, bias);
 }
@@ -143,22 +152,29 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
     T *dx = (T *)a.dx + (long)b * a.L * a.C + c;
     // dx of position t - K + 1 is complete once g_t is known; the first stretch also gives the carried state's gradient
     const T *x = (const T *)a.x + b * a.xb + c;
-    for (long tb0 = t0; tb0 < t1 + K - 1; tb0 += BWD_UNDER) {
-    RawVec<T, V> rx[BWD_UNDER], rg[BWD_UNDER];  // so many positions are under way at once
+    struct Block {
+      RawVec<T, V> x[BWD_UNDER], g[BWD_UNDER];
+    } cur, next;
+    auto fetch = [&](long from) {
 #pragma unroll
-    for (int j = 0; j < BWD_UNDER; ++j) {
-      const long t = tb0 + j < a.L ? tb0 + j : a.L - 1;
-      rx[j].load(x + t * a.xt);
-      rg[j].load(dy + t * a.dyt);
-    }
+      for (int j = 0; j < BWD_UNDER; ++j) {
+        const long t = from + j < a.L ? from + j : a.L - 1;
+        next.x[j].load(x + t * a.xt);
+        next.g[j].load(dy + t * a.dyt);
+      }
+    };
+    fetch(t0);
+    for (long tb0 = t0; tb0 < t1 + K - 1; tb0 += BWD_UNDER) {
+    cur = next;
+    if (tb0 + BWD_UNDER < t1 + K - 1) fetch(tb0 + BWD_UNDER);
 #pragma unroll
     for (int j = 0; j < BWD_UNDER; ++j) {
       const long t = tb0 + j;
       if (t >= t1 + K - 1) break;
       if (t < len) {
         float d[V];
-        rx[j].get(true, h[K - 1]);
-        rg[j].get(true, d);
+        cur.x[j].get(true, h[K - 1]);
+        cur.g[j].get(true, d);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if (a.silu) {
@@ -288,7 +304,7 @@ extern "C" int bkcore_causal_conv(const void *x, int64_t x_batch, int64_t x_time
   ConvArgs a{};
   a.x = x; a.w = weight; a.bias = bias; a.init = initial_state; a.y = y; a.final_state = final_state;
   a.lengths = lengths; a.xb = x_batch; a.xt = x_time; a.B = (int)B; a.L = (int)L; a.C = (int)C;
-  a.param_f32 = param_dtype == BKCORE_F32; a.silu = silu != 0;
+  a.param_f32 = param_dtype == BKCORE_F32; a.param_vec = a.param_f32 && aligned16(weight); a.silu = silu != 0;
   const int64_t nseg = L > 0 ? (L + FWD_TL - 1) / FWD_TL : 1, nvec = vec ? C / v : C;
   const int64_t blocks = (B * nseg * nvec + 255) / 256;
   if (blocks > 2147483647LL) return BKCORE_EINVAL;
@@ -327,7 +343,7 @@ extern "C" int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int
   a.x = x; a.w = weight; a.bias = bias; a.init = initial_state; a.dy = dy; a.dfinal = grad_final_state;
   a.dx = dx; a.dinit = grad_initial_state; a.part = grad_params ? (float *)workspace : nullptr; a.lengths = lengths;
   a.xb = x_batch; a.xt = x_time; a.dyb = dy_batch; a.dyt = dy_time; a.B = (int)B; a.L = (int)L; a.C = (int)C;
-  a.param_f32 = param_dtype == BKCORE_F32; a.silu = silu != 0;
+  a.param_f32 = param_dtype == BKCORE_F32; a.param_vec = a.param_f32 && aligned16(weight); a.silu = silu != 0;
   const int64_t nblk = backward_blocks(L), nvec = vec ? C / v : C, cblk = (nvec + BWD_CH - 1) / BWD_CH;
   if (B * nblk * cblk > 2147483647LL) return BKCORE_EINVAL;
 #define BK_CONV(K_, V_)                                                                                              \
@@ -351,7 +367,7 @@ extern "C" int bkcore_causal_conv_step(const void *x, int64_t x_batch, int dtype
   const bool vec = C % v == 0 && x_batch % v == 0 && aligned16(x) && aligned16(y) && aligned16(state);
   ConvArgs a{};
   a.x = x; a.w = weight; a.bias = bias; a.y = y; a.xb = x_batch; a.B = (int)B; a.L = 1; a.C = (int)C;
-  a.param_f32 = param_dtype == BKCORE_F32; a.silu = silu != 0;
+  a.param_f32 = param_dtype == BKCORE_F32; a.param_vec = a.param_f32 && aligned16(weight); a.silu = silu != 0;
   const int64_t nvec = vec ? C / v : C, blocks = (B * nvec + 255) / 256;
   if (blocks > 2147483647LL) return BKCORE_EINVAL;
 #define BK_CONV(K_, V_)                                                                                              \
