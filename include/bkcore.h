@@ -428,6 +428,48 @@ int bkcore_selective_scan_step(const void *x, int64_t x_batch, float *state, con
                                const float *D, const void *z, int64_t z_batch, const float *delta_bias,
                                int softplus_delta, int dtype, int64_t B, int64_t C, int64_t N, void *y, void *stream);
 
+/* Causal softmax attention in a sliding window with sinks: query i of a sequence sees keys j <= i with i - j < window or
+ * j < sinks (the first tokens, at most 64), H query heads over Hk key / value heads (H a multiple of Hk; neighbouring query
+ * heads share one).  Takes the place of the windowed local path (src/models/phase7/hybrid_attention.py:93-103), whose
+ * windows are blocks.  q (B, H, L, D), k, v (B, Hk, L, D) by strides, D <= 128; out (B, L, H, D) contiguous; lse: NULL, or
+ * (B, H, L) floats for the backward (base-2 logarithm of the row's sum; +inf for a row that sees nothing). */
+#define BKCORE_ATTENTION_MAX_HEAD_DIM 128
+#define BKCORE_ATTENTION_MAX_SINKS 64
+int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t q_head, int64_t q_time, const void *k,
+                             int64_t k_batch, int64_t k_head, int64_t k_time, const void *v, int64_t v_batch,
+                             int64_t v_head, int64_t v_time, int dtype, const int *lengths, int64_t B, int64_t H, int64_t Hk,
+                             int64_t L, int64_t D, int64_t window, int64_t sinks, float scale, void *out, float *lse,
+                             void *stream);
+/* dq (B, L, H, D), dk, dv (B, L, Hk, D) contiguous; sums in a fixed order (no atomics). */
+size_t bkcore_sliding_attention_backward_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D,
+                                                         int64_t window, int64_t sinks);
+int bkcore_sliding_attention_backward(const void *dout, int64_t do_batch, int64_t do_head, int64_t do_time, const void *q,
+                                      int64_t q_batch, int64_t q_head, int64_t q_time, const void *k, int64_t k_batch,
+                                      int64_t k_head, int64_t k_time, const void *v, int64_t v_batch, int64_t v_head,
+                                      int64_t v_time, const void *out, const float *lse, int dtype, const int *lengths,
+                                      int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D, int64_t window, int64_t sinks,
+                                      float scale, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                                      void *stream);
+/* One token of each sequence: appends k, v (B, Hk, D) to a rolling cache of cap >= window + sinks slots and attends with
+ * q (B, H, D).  positions: B ints on the device, the new token's position; a negative one leaves its sequence alone (output
+ * zero, cache as it was).  Position p lives in slot p for p < sinks and in slot sinks + (p - sinks) % (cap - sinks) behind.
+ * out (B, H, D) contiguous.  The workspace is needed when its size is not zero. */
+size_t bkcore_sliding_attention_step_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t cap, int64_t D,
+                                                     int64_t window, int64_t sinks);
+int bkcore_sliding_attention_step(const void *q, int64_t q_batch, int64_t q_head, const void *k, int64_t k_batch,
+                                  int64_t k_head, const void *v, int64_t v_batch, int64_t v_head, void *k_cache,
+                                  int64_t kc_batch, int64_t kc_head, int64_t kc_slot, void *v_cache, int64_t vc_batch,
+                                  int64_t vc_head, int64_t vc_slot, const int *positions, int dtype, int64_t B, int64_t H,
+                                  int64_t Hk, int64_t cap, int64_t D, int64_t window, int64_t sinks, float scale, void *out,
+                                  void *workspace, size_t workspace_bytes, void *stream);
+/* Fills such a cache from a prompt's k, v (B, Hk, L, D): the sinks and the last cap - sinks positions behind them; other
+ * slots stay as they were. */
+int bkcore_sliding_cache_fill(const void *k, int64_t k_batch, int64_t k_head, int64_t k_time, const void *v,
+                              int64_t v_batch, int64_t v_head, int64_t v_time, void *k_cache, int64_t kc_batch,
+                              int64_t kc_head, int64_t kc_slot, void *v_cache, int64_t vc_batch, int64_t vc_head,
+                              int64_t vc_slot, const int *lengths, int dtype, int64_t B, int64_t Hk, int64_t L, int64_t cap,
+                              int64_t D, int64_t sinks, void *stream);
+
 /* Largest N bkcore_forward accepts. */
 int64_t bkcore_max_seq_len(void);
 

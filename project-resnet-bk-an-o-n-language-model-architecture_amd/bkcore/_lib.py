@@ -36,6 +36,9 @@ EXPORTS = ("bkcore_forward", "bkcore_forward_clamped", "bkcore_forward_noalloc",
            "bkcore_causal_conv_step", "bkcore_selective_scan", "bkcore_selective_scan_workspace_bytes",
            "bkcore_selective_scan_checkpoint_bytes", "bkcore_selective_scan_backward",
            "bkcore_selective_scan_backward_workspace_bytes", "bkcore_selective_scan_step",
+           "bkcore_sliding_attention", "bkcore_sliding_attention_backward",
+           "bkcore_sliding_attention_backward_workspace_bytes", "bkcore_sliding_attention_step",
+           "bkcore_sliding_attention_step_workspace_bytes", "bkcore_sliding_cache_fill",
            "bkcore_max_seq_len", "bkcore_forward_plan", "bkcore_last_hip_error",
            "bkcore_error_string", "bkcore_abi_version")
 
@@ -148,12 +151,19 @@ def _declare(L):
                                         i64, i64, vp, i32, i32, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp,
                                         sz, vp],
             "selective_scan_step": [vp, i64, vp, vp, i64, vp, vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i64, i64, i64, vp,
-                                    vp]}.items():
+                                    vp],
+            "sliding_attention": [vp, i64, i64, i64] * 3 + [i32, vp] + [i64] * 7 + [f32, vp, vp, vp],
+            "sliding_attention_backward": [vp, i64, i64, i64] * 4 + [vp, vp, i32, vp] + [i64] * 7 + [f32, vp, vp, vp, vp, sz,
+                                                                                                  vp],
+            "sliding_attention_step": [vp, i64, i64] * 3 + [vp, i64, i64, i64] * 2 + [vp, i32] + [i64] * 7 + [f32, vp, vp, sz,
+                                                                                                            vp],
+            "sliding_cache_fill": [vp, i64, i64, i64] * 4 + [vp, i32] + [i64] * 6 + [vp]}.items():
         fn = getattr(L, "bkcore_" + name)
         fn.argtypes, fn.restype = args, i32
     for name, n in {"layer_norm_backward_workspace_bytes": 2, "causal_conv_backward_workspace_bytes": 4,
                     "selective_scan_workspace_bytes": 4, "selective_scan_checkpoint_bytes": 4,
-                    "selective_scan_backward_workspace_bytes": 4}.items():
+                    "selective_scan_backward_workspace_bytes": 4, "sliding_attention_backward_workspace_bytes": 7,
+                    "sliding_attention_step_workspace_bytes": 7}.items():
         fn = getattr(L, "bkcore_" + name)
         fn.argtypes, fn.restype = [i64] * n, sz
     L.bkcore_max_seq_len.restype = i64

@@ -1,0 +1,185 @@
+"""Causal attention in a sliding window with sinks (a few first tokens that stay visible): the local mixing path of the
+hybrid layer without its block borders (reference src/models/phase7/hybrid_attention.py:93-103), for training, for prompts
+and, on a rolling key / value cache, for single tokens.
+
+Query i of a sequence sees the keys j <= i with ``i - j < window`` or ``j < sinks``.  Positions at or behind ``lengths``
+(B,) are padding of a right-padded batch: they are never read, outputs and gradients there are zero."""
+from __future__ import annotations
+
+import torch
+
+from . import _layer_ops as ops
+from . import _lib
+
+MAX_HEAD_DIM = 128   # BKCORE_ATTENTION_MAX_HEAD_DIM
+MAX_SINKS = 64       # BKCORE_ATTENTION_MAX_SINKS
+
+
+def _window(what: str, window, sinks) -> tuple[int, int]:
+    window, sinks = int(window), int(sinks)
+    if window < 1:
+        raise ValueError(f"bkcore: {what}: a window holds at least one position, got {window}")
+    if not 0 <= sinks <= MAX_SINKS:
+        raise ValueError(f"bkcore: {what}: 0 to {MAX_SINKS} sinks, got {sinks}")
+    return window, sinks
+
+
+def _heads(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dims: int) -> int:
+    """Checks q (B, H, ...), k and v (B, Hk, ...) and returns the type's code."""
+    ops.need_device(q, k, v)
+    code = ops.need_dtype(what, q, k, v)
+    if q.dim() != dims or k.dim() != dims or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError(f"bkcore: {what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if q.shape[1] < 1 or k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"bkcore: {what}: {q.shape[1]} query heads are no multiple of {k.shape[1]} key heads")
+    if not 1 <= q.shape[-1] <= MAX_HEAD_DIM:
+        raise ValueError(f"bkcore: {what}: head dimensions 1 to {MAX_HEAD_DIM}, got {q.shape[-1]}")
+    return code
+
+
+def _scale(what: str, scale, D: int) -> float:
+    scale = D ** -0.5 if scale is None else float(scale)
+    if scale != scale:
+        raise ValueError(f"bkcore: {what}: scale is not a number")
+    return scale
+
+
+class _SlidingAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale, lengths, keep):
+        q, k, v = ops.inner(q), ops.inner(k), ops.inner(v)
+        B, H, T, D = q.shape
+        Hk = k.shape[1]
+        dev = q.device
+        o = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
+        lse = torch.empty(B * H * T, dtype=torch.float32, device=dev) if keep else None
+        with ops.on_device(dev):
+            rc = _lib.load_held().bkcore_sliding_attention(
+                q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+                ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window, sinks, scale, o.data_ptr(), ops.ptr(lse),
+                ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_sliding_attention")
+        if keep:
+            ctx.save_for_backward(q, k, v, o, lse, lengths)
+            ctx.bk_args = window, sinks, scale
+        return o.transpose(1, 2)
+
+    @staticmethod
+    def backward(ctx, do):
+        ops.once_only("sliding_attention")
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        window, sinks, scale = ctx.bk_args
+        do = ops.inner(do)
+        B, H, T, D = q.shape
+        Hk = k.shape[1]
+        dev = q.device
+        dq = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
+        dk = torch.empty(B, T, Hk, D, dtype=q.dtype, device=dev)
+        dv = torch.empty_like(dk)
+        L = _lib.load_held()
+        nbytes = L.bkcore_sliding_attention_backward_workspace_bytes(B, H, Hk, T, D, window, sinks)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with ops.on_device(dev):
+            rc = L.bkcore_sliding_attention_backward(
+                do.data_ptr(), *do.stride()[:3], q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+                *v.stride()[:3], o.data_ptr(), lse.data_ptr(), ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window,
+                sinks, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes, ops.stream(dev.index))
+        if rc:
+            _lib.check(rc, "bkcore_sliding_attention_backward")
+        need = ctx.needs_input_grad
+        return (dq.transpose(1, 2) if need[0] else None, dk.transpose(1, 2) if need[1] else None,
+                dv.transpose(1, 2) if need[2] else None, None, None, None, None, None)
+
+
+def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                      scale: float | None = None, lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q (B, H, L, D) to k, v (B, Hk, L, D) of the same positions, H a multiple of Hk (neighbouring query heads
+    share a key / value head), D <= 128, at most 64 sinks; ``scale`` defaults to D ** -0.5.  Heads and positions may have any
+    strides (slices of one projection).  The result (B, H, L, D) has its heads inside a position in memory.
+
+    Scores, softmax and sums are float32; probabilities enter the product with v in the operands' type.  A non-finite key
+    or value inside a sequence may reach any row that works on the same tile of keys, not only those that see it."""
+    what = "sliding_attention"
+    _heads(what, q, k, v, 4)
+    B, H, T, D = q.shape
+    window, sinks = _window(what, window, sinks)
+    scale = _scale(what, scale, D)
+    n = ops.lengths_arg(what, lengths, q, B, T)
+    return _SlidingAttentionFunction.apply(q, k, v, window, sinks, scale, n, ops.wants_grad(q, k, v))
+
+
+def _cache(what: str, q: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int) -> int:
+    """Checks the caches (B, Hk, slots, D) and returns the number of slots."""
+    ops.need_device(q, k_cache, v_cache)
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.dim() != 4 or c.shape[:2] != k.shape[:2] or c.shape[3] != k.shape[-1] or c.shape != k_cache.shape:
+            raise ValueError(f"bkcore: {what}: {name} is (B, Hk, slots, D), got {tuple(c.shape)}")
+        if c.shape[3] > 1 and c.stride(3) != 1:
+            raise ValueError(f"bkcore: {what}: the last dimension of {name} must be contiguous")
+        if c.shape[2] > 1 and c.stride(2) < c.shape[3]:
+            raise ValueError(f"bkcore: {what}: the slots of {name} overlap")
+        ops.need_state(what, name, c, q, tuple(c.shape), q.dtype)
+    if k_cache.shape[2] <= sinks:
+        raise ValueError(f"bkcore: {what}: {k_cache.shape[2]} slots leave none behind {sinks} sinks")
+    return k_cache.shape[2]
+
+
+def sliding_cache_fill(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       lengths: torch.Tensor | None = None, sinks: int = 0) -> None:
+    """Writes a prompt's keys and values (B, Hk, L, D) into rolling caches (B, Hk, slots, D): the first ``sinks`` positions
+    and the last ``slots - sinks`` behind them.  Position p lives in slot p for p < sinks and in slot
+    ``sinks + (p - sinks) % (slots - sinks)`` behind; slots of no position stay as they were."""
+    what = "sliding_cache_fill"
+    code = _heads(what, k, k, v, 4)
+    _, sinks = _window(what, 1, sinks)
+    ops.no_grad_through(what, k, v)
+    cap = _cache(what, k, k, k_cache, v_cache, sinks)
+    B, Hk, T, D = k.shape
+    n = ops.lengths_arg(what, lengths, k, B, T)
+    k, v = ops.inner(k), ops.inner(v)
+    dev = k.device
+    with ops.on_device(dev):
+        rc = _lib.load_held().bkcore_sliding_cache_fill(
+            k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], k_cache.data_ptr(), *k_cache.stride()[:3],
+            v_cache.data_ptr(), *v_cache.stride()[:3], ops.ptr(n), code, B, Hk, T, cap, D, sinks, ops.stream(dev.index))
+    if rc:
+        _lib.check(rc, "bkcore_sliding_cache_fill")
+
+
+def sliding_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           positions: torch.Tensor, window: int, sinks: int = 0,
+                           scale: float | None = None) -> torch.Tensor:
+    """``sliding_attention`` for one token of each sequence: q (B, H, D), k and v (B, Hk, D) of the token at ``positions``
+    (B,), which are written into the rolling caches (see ``sliding_cache_fill``; at least ``window + sinks`` slots) in place.
+    A negative position leaves its sequence alone: output zero, cache as it was.  No gradient."""
+    what = "sliding_attention_step"
+    code = _heads(what, q, k, v, 3)
+    window, sinks = _window(what, window, sinks)
+    ops.no_grad_through(what, q, k, v)
+    cap = _cache(what, q, k, k_cache, v_cache, sinks)
+    if cap < window + sinks:
+        raise ValueError(f"bkcore: {what}: a window of {window} and {sinks} sinks need {window + sinks} slots, got {cap}")
+    B, H, D = q.shape
+    Hk = k.shape[1]
+    scale = _scale(what, scale, D)
+    ops.need_shape(what, "positions", positions, (B,))
+    ops.need_device(q, positions)
+    if positions.dtype == torch.int64:
+        positions = positions.to(torch.int32)
+    elif positions.dtype != torch.int32:
+        raise TypeError(f"bkcore: {what}: positions are int32 or int64, not {positions.dtype}")
+    q, k, v, positions = ops.inner(q), ops.inner(k), ops.inner(v), positions.contiguous()
+    dev = q.device
+    o = torch.empty(B, H, D, dtype=q.dtype, device=dev)
+    L = _lib.load_held()
+    nbytes = L.bkcore_sliding_attention_step_workspace_bytes(B, H, Hk, cap, D, window, sinks)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with ops.on_device(dev):
+        rc = L.bkcore_sliding_attention_step(
+            q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], k_cache.data_ptr(),
+            *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], positions.data_ptr(), code, B, H, Hk, cap, D,
+            window, sinks, scale, o.data_ptr(), ops.ptr(ws), nbytes, ops.stream(dev.index))
+    if rc:
+        _lib.check(rc, "bkcore_sliding_attention_step")
+    return o

@@ -1,0 +1,880 @@
+// Kernels of sliding-window attention with sinks, instantiated for one operand type by the file that includes this one.
+//   s_ij = scale q_i . k_j for j <= i with i - j < W or j < S;  o_i = sum_j p_ij v_j,  p_ij = exp(s_ij) / sum_j exp(s_ij)
+//   backward, delta_i = do_i . o_i:  ds_ij = p_ij (do_i . v_j - delta_i);  dq_i = scale sum_j ds_ij k_j;
+//   dk_j = scale sum_i ds_ij q_i;  dv_j = sum_i p_ij do_i   (sums over the query heads that share the key's head)
+//
+// All products go to the 16 x 16 matrix instructions.  A fragment is eight elements a lane: for 16-bit operands one
+// instruction of depth 32, for float32 eight of depth 4 on the same registers (the order of the contracted index is free as
+// long as both operands agree), so one body serves all types.  Scores are formed transposed (keys x queries): a lane then
+// holds four neighbouring keys of one query, which is the layout the next product wants its second operand in -- the
+// probabilities go from accumulators to operands without leaving the lane, and the row's maximum and sum are a lane's own
+// plus two exchanges.  The other operand of that product (V, or K, Q, dO in the backward) is contracted over its rows: it
+// is read from LDS through the transposing read (16-bit) or element by element (float32).
+#include "bkcore_attention.h"
+
+namespace bk {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Frag {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec v;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+  } else if constexpr (__is_same(T, bf16_t)) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
+  }
+}
+
+template <typename T>
+constexpr int pad() { return 16 / (int)sizeof(T); }  // elements that set LDS rows apart: 16 rows then cover all 64 banks
+
+// Eight elements of row `row` (clamped by the caller to one that exists) from column c: raw, zeroed where not wanted.
+template <typename T, bool VEC>
+__device__ __forceinline__ Frag<T> load8(const T *row, int c, int D) {
+  Frag<T> f;
+  if constexpr (VEC) {
+    f.v = *reinterpret_cast<const typename Frag<T>::vec *>(row + (c < D ? c : 0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = row[c + i < D ? c + i : 0];
+  }
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> zero_unless(const Frag<T> &f, bool row_ok, int c, int D) {
+  Frag<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = row_ok && c + i < D ? f.v[i] : (T)0.0f;
+  return r;
+}
+
+// ROWS x DP elements on their way from memory to LDS (row stride DP + pad), THREADS threads.
+template <typename T, int ROWS, int DP, int THREADS, bool VEC>
+struct Tile {
+  static constexpr int CH = DP / 8, N = (ROWS * CH + THREADS - 1) / THREADS;
+  static constexpr bool WHOLE = ROWS * CH % THREADS == 0;  // else the last pass is for some of the threads
+  Frag<T> r[N];
+  __device__ __forceinline__ void load(const T *base, long stride, long row0, long rows, int D, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = tid + k * THREADS;
+      long row = row0 + i / CH;
+      row = row < rows ? row : rows - 1;
+      r[k] = load8<T, VEC>(base + row * stride, (i % CH) * 8, D);
+    }
+  }
+  __device__ __forceinline__ void store(T *lds, long row0, long rows, int D, int tid) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = tid + k * THREADS, row = i / CH, c = (i % CH) * 8;
+      if (!WHOLE && i >= ROWS * CH) break;
+      const Frag<T> f = zero_unless(r[k], row0 + row < rows, c, D);
+      *reinterpret_cast<typename Frag<T>::vec *>(lds + row * (DP + pad<T>()) + c) = f.v;
+    }
+  }
+};
+
+// Operand whose contracted index runs along the row: element i of lane l is row l % 16, column 8 (l / 16) + i.
+template <typename T, int DP>
+__device__ __forceinline__ Frag<T> along(const T *lds, int row0, int col0, int lane) {
+  Frag<T> f;
+  f.v = *reinterpret_cast<const typename Frag<T>::vec *>(lds + (row0 + (lane & 15)) * (DP + pad<T>()) + col0 + (lane >> 4) * 8);
+  return f;
+}
+
+// Operand contracted over rows: lane l holds column col0 + l % 16 of rows row0 + 4 g + (0..3) and row0 + 16 + 4 g + (0..3),
+// g = l / 16 -- the order in which two 16-row score blocks leave their accumulators.
+template <typename T, int DP>
+__device__ __forceinline__ Frag<T> across(const T *lds, int row0, int col0, int lane) {
+  constexpr int LD = DP + pad<T>();
+  const int g = lane >> 4, m = lane & 15;
+  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) s16x4 lds_vec;
+    const T *p = lds + (row0 + 4 * g + (m >> 2)) * LD + col0 + 4 * (m & 3);
+    union {
+      s16x4 s[2];
+      typename Frag<T>::vec v;
+    } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec *)p);
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_vec *)(p + 16 * LD));
+    f.v = u.v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = lds[(row0 + 4 * g + (i & 3) + 16 * (i >> 2)) * LD + col0 + m];
+  }
+  return f;
+}
+
+// Two 16-row blocks of a score column as one operand, rounded to the operands' type: probabilities and their gradients
+// enter the second product in the precision of the values they multiply, the sum of the probabilities stays float32.
+template <typename T>
+__device__ __forceinline__ Frag<T> to_frag(const f32x4 &lo, const f32x4 &hi) {
+  Frag<T> f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f.v[i] = (T)lo[i];
+    f.v[4 + i] = (T)hi[i];
+  }
+  return f;
+}
+
+// Maximum / sum over the four lanes that hold one column (l, l + 16, l + 32, l + 48), in each of them.
+__device__ __forceinline__ float col_max(float x) {
+  u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float col_sum(float x) {
+  x = fold16(x, x);
+  return fold32(x, x);
+}
+
+__device__ __forceinline__ int row_length(const int *lengths, int b, int L) {
+  if (!lengths) return L;
+  const int n = lengths[b];
+  return n < 0 ? 0 : n > L ? L : n;
+}
+
+constexpr float INF = __builtin_inff();
+
+// Work item of a workgroup: neighbouring items share keys and values, so each of the eight dies gets a contiguous run of
+// them (workgroups go to the dies in turn).  -1: none left.
+__device__ __forceinline__ long work_item(long total) {
+  const long per = (total + 7) / 8, w = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  return (long)(blockIdx.x >> 3) < per && w < total ? w : -1;
+}
+inline unsigned work_grid(long total) { return (unsigned)((total + 7) / 8 * 8); }
+
+template <typename T>
+__device__ __forceinline__ const T *head(const Heads &x, int b, int h) {
+  return (const T *)x.p + b * x.b + h * x.h;
+}
+
+// Four neighbouring d of a row (of a (B, L, heads, D) result), rounded to T.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T *row, int d, int D, const f32x4 &v) {
+  if constexpr (VEC) {
+    if (d < D) {
+      typedef T vec4 __attribute__((ext_vector_type(4)));
+      vec4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (T)v[i];
+      *reinterpret_cast<vec4 *>(row + d) = w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < D) row[d + i] = (T)v[i];
+  }
+}
+
+// Keys of a tile: 64 for 16-bit operands, 32 for float32 (registers on the way to LDS).
+template <typename T>
+constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+
+// The tiles of keys that queries [q0, q1] see: first those that hold only sinks, then the window's.
+struct KeyTiles {
+  int nsink, first, n;
+  __device__ __forceinline__ KeyTiles(int q0, int q1, int W, int S, int BN) {
+    const int lo = q0 - W + 1 > 0 ? q0 - W + 1 : 0;
+    first = lo / BN;
+    const int s = (S + BN - 1) / BN;
+    nsink = s < first ? s : first;
+    n = q1 >= q0 ? nsink + q1 / BN - first + 1 : 0;
+  }
+  __device__ __forceinline__ int key0(int i, int BN) const { return (i < nsink ? i : first + i - nsink) * BN; }
+};
+
+// What queries [q0, q1] see of keys [j0, j1]: 0 nothing, 1 some, 2 everything.
+__device__ __forceinline__ int tile_view(int q0, int q1, int j0, int j1, int W, int S) {
+  if (j0 > q1 || (q0 - j1 >= W && j0 >= S)) return 0;
+  return j1 <= q0 && (q1 - j0 < W || j1 < S) ? 2 : 1;
+}
+__device__ __forceinline__ bool sees(int i, int j, int W, int S) { return j <= i && (i - j < W || j < S); }
+
+// ---- forward: 4 waves x 32 queries; keys and values through LDS, the next tile on its way in registers.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256) void bk_attn_kernel(AttnArgs a) {
+  constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32;
+  __shared__ __attribute__((aligned(16))) T sK[BN * LD], sV[BN * LD];
+  const int nq = (a.L + ATTN_BM - 1) / ATTN_BM;
+  long w = work_item((long)a.B * a.H * nq);
+  if (w < 0) return;
+  const int G = a.H / a.Hk;
+  const int g_ = (int)(w % G);
+  w /= G;
+  const int qt = (int)(w % nq);
+  w /= nq;
+  const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), h = hk * G + g_;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int len = row_length(a.lengths, b, a.L);
+  const int q0 = qt * ATTN_BM, q1 = min(q0 + ATTN_BM, len) - 1;
+  const int w0 = q0 + wave * 32, w1 = min(w0 + 32, len) - 1;  // the wave's own queries
+  const T *qp = head<T>(a.q, b, h), *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
+  const float sc = a.scale * LOG2E;
+
+  Frag<T> q[2][NC];
+  if (q1 >= q0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = w0 + 16 * i + m;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        q[i][c] = load8<T, VEC>(qp + (long)min(row, len - 1) * a.q.t, c * 32 + g * 8, a.D);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) q[i][c] = zero_unless(q[i][c], row < len, c * 32 + g * 8, a.D);
+    }
+  }
+  f32x4 o[ND][2];
+  float mx[2], sum[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    mx[i] = -INF;
+    sum[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d][i] = {0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const KeyTiles kt(q0, q1, a.W, a.S, BN);
+  Tile<T, BN, DP, 256, VEC> tk, tv;
+  if (kt.n) {
+    tk.load(kp, a.k.t, kt.key0(0, BN), len, a.D, tid);
+    tv.load(vp, a.v.t, kt.key0(0, BN), len, a.D, tid);
+  }
+  for (int it = 0; it < kt.n; ++it) {
+    const int j0 = kt.key0(it, BN);
+    __syncthreads();
+    tk.store(sK, j0, len, a.D, tid);
+    tv.store(sV, j0, len, a.D, tid);
+    __syncthreads();
+    if (it + 1 < kt.n) {
+      const int j = kt.key0(it + 1, BN);
+      tk.load(kp, a.k.t, j, len, a.D, tid);
+      tv.load(vp, a.v.t, j, len, a.D, tid);
+    }
+    const int view = w1 >= w0 ? tile_view(w0, w1, j0, j0 + BN - 1, a.W, a.S) : 0;
+    if (!view) continue;
+    f32x4 s[NK][2];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      s[k][0] = s[k][1] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const Frag<T> kf = along<T, DP>(sK, 16 * k, 32 * c, lane);
+        mma(kf, q[0][c], s[k][0]);
+        mma(kf, q[1][c], s[k][1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int qi = w0 + 16 * i + m;
+      float top = -INF;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = s[k][i][r] * sc;
+          if (view == 1) x = sees(qi, j0 + 16 * k + 4 * g + r, a.W, a.S) ? x : -INF;
+          s[k][i][r] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(mx[i], col_max(top));
+      const float ref = top == -INF ? 0.0f : top, alpha = exp2_fast(mx[i] - ref);
+      mx[i] = top;
+      float part = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[k][i][r] = exp2_fast(s[k][i][r] - ref);
+          part += s[k][i][r];
+        }
+      sum[i] = fmaf(sum[i], alpha, part);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[d][i][r] *= alpha;
+    }
+#pragma unroll
+    for (int k = 0; k < NK; k += 2) {
+      const Frag<T> p0 = to_frag<T>(s[k][0], s[k + 1][0]), p1 = to_frag<T>(s[k][1], s[k + 1][1]);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const Frag<T> vf = across<T, DP>(sV, 16 * k, 16 * d, lane);
+        mma(vf, p0, o[d][0]);
+        mma(vf, p1, o[d][1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = w0 + 16 * i + m;
+    const float l = col_sum(sum[i]);
+    if (row < a.L) {
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // a row that sees nothing: zeros
+      T *op = (T *)a.o + (((long)b * a.L + row) * a.H + h) * a.D;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = row < len ? o[d][i][r] * inv : 0.0f;
+        store4<T, VEC>(op, 16 * d + 4 * g, a.D, v);
+      }
+      if (a.lse && g == 0)
+        a.lse[((long)b * a.H + h) * a.L + row] =
+            row < len && (l > 0.0f || l != l) ? mx[i] + __builtin_amdgcn_logf(l) : INF;
+    }
+  }
+}
+
+// ---- delta_i = do_i . o_i, one wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void bk_attn_delta_kernel(AttnArgs a) {
+  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (id >= (long)a.B * a.L * a.H) return;
+  const int h = (int)(id % a.H);
+  const long bt = id / a.H;
+  const int b = (int)(bt / a.L), t = (int)(bt % a.L);
+  float s = 0.0f;
+  if (t < row_length(a.lengths, b, a.L)) {
+    const T *o = (const T *)a.out + id * a.D, *g = head<T>(a.dout, b, h) + (long)t * a.dout.t;
+    for (int d = lane; d < a.D; d += 64) s = fmaf((float)o[d], (float)g[d], s);
+  }
+  s = wave_sum(s);
+  if (lane == 0) a.delta[((long)b * a.H + h) * a.L + t] = s;
+}
+
+// ---- dq: the forward's loop with two score products, dS^T in the lane, and K contracted over its rows.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256) void bk_attn_dq_kernel(AttnArgs a) {
+  constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32;
+  __shared__ __attribute__((aligned(16))) T sK[BN * LD], sV[BN * LD];
+  const int nq = (a.L + ATTN_BM - 1) / ATTN_BM;
+  long w = work_item((long)a.B * a.H * nq);
+  if (w < 0) return;
+  const int G = a.H / a.Hk;
+  const int g_ = (int)(w % G);
+  w /= G;
+  const int qt = (int)(w % nq);
+  w /= nq;
+  const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), h = hk * G + g_;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int len = row_length(a.lengths, b, a.L);
+  const int q0 = qt * ATTN_BM, q1 = min(q0 + ATTN_BM, len) - 1;
+  const int w0 = q0 + wave * 32, w1 = min(w0 + 32, len) - 1;
+  const T *qp = head<T>(a.q, b, h), *gp = head<T>(a.dout, b, h), *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
+  const float sc = a.scale * LOG2E;
+  Frag<T> q[2][NC], go[2][NC];
+  float lse[2], delta[2];
+  f32x4 dq[ND][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = w0 + 16 * i + m;
+    lse[i] = INF;
+    delta[i] = 0.0f;
+    if (q1 >= q0) {
+      const long r = min(row, len - 1);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        q[i][c] = load8<T, VEC>(qp + r * a.q.t, c * 32 + g * 8, a.D);
+        go[i][c] = load8<T, VEC>(gp + r * a.dout.t, c * 32 + g * 8, a.D);
+      }
+      const float l_ = a.lse[((long)b * a.H + h) * a.L + r], d_ = a.delta[((long)b * a.H + h) * a.L + r];
+      if (row < len) {
+        lse[i] = l_;
+        delta[i] = d_;
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        q[i][c] = zero_unless(q[i][c], row < len, c * 32 + g * 8, a.D);
+        go[i][c] = zero_unless(go[i][c], row < len, c * 32 + g * 8, a.D);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dq[d][i] = {0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const KeyTiles kt(q0, q1, a.W, a.S, BN);
+  Tile<T, BN, DP, 256, VEC> tk, tv;
+  if (kt.n) {
+    tk.load(kp, a.k.t, kt.key0(0, BN), len, a.D, tid);
+    tv.load(vp, a.v.t, kt.key0(0, BN), len, a.D, tid);
+  }
+  for (int it = 0; it < kt.n; ++it) {
+    const int j0 = kt.key0(it, BN);
+    __syncthreads();
+    tk.store(sK, j0, len, a.D, tid);
+    tv.store(sV, j0, len, a.D, tid);
+    __syncthreads();
+    if (it + 1 < kt.n) {
+      const int j = kt.key0(it + 1, BN);
+      tk.load(kp, a.k.t, j, len, a.D, tid);
+      tv.load(vp, a.v.t, j, len, a.D, tid);
+    }
+    const int view = w1 >= w0 ? tile_view(w0, w1, j0, j0 + BN - 1, a.W, a.S) : 0;
+    if (!view) continue;
+#pragma unroll
+    for (int k = 0; k < NK; k += 2) {
+      f32x4 s[2][2], dp[2][2];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        s[kk][0] = s[kk][1] = dp[kk][0] = dp[kk][1] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const Frag<T> kf = along<T, DP>(sK, 16 * (k + kk), 32 * c, lane), vf = along<T, DP>(sV, 16 * (k + kk), 32 * c, lane);
+          mma(kf, q[0][c], s[kk][0]);
+          mma(kf, q[1][c], s[kk][1]);
+          mma(vf, go[0][c], dp[kk][0]);
+          mma(vf, go[1][c], dp[kk][1]);
+        }
+      }
+      Frag<T> ds[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int qi = w0 + 16 * i + m;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p = exp2_fast(fmaf(s[kk][i][r], sc, -lse[i]));
+            float x = p * (dp[kk][i][r] - delta[i]);
+            if (view == 1) x = sees(qi, j0 + 16 * (k + kk) + 4 * g + r, a.W, a.S) ? x : 0.0f;
+            s[kk][i][r] = x;
+          }
+        ds[i] = to_frag<T>(s[0][i], s[1][i]);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const Frag<T> kf = across<T, DP>(sK, 16 * k, 16 * d, lane);
+        mma(kf, ds[0], dq[d][0]);
+        mma(kf, ds[1], dq[d][1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = w0 + 16 * i + m;
+    if (row < a.L) {
+      T *op = (T *)a.dq + (((long)b * a.L + row) * a.H + h) * a.D;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = row < len && lse[i] != INF ? dq[d][i][r] * a.scale : 0.0f;
+        store4<T, VEC>(op, 16 * d + 4 * g, a.D, v);
+      }
+    }
+  }
+}
+
+// ---- dk, dv.  SINK false: 4 waves x 32 keys, all of them over the same 32 queries at a time, over the tile's own queries
+// (its window) and the heads of the group.  SINK true: the sinks' part behind that -- the first 64 keys see all later
+// queries, so their loop is the whole sequence: it is cut into stretches, a wave takes 32 keys (keys 32 kh ...) and its own
+// 32 of every 128 queries, and leaves float32 sums that the join adds up in a fixed order.
+// part: (1 + 4 nsplit, B, Hk, S, 2, D); slot 0 is what the first key tile has from its own queries.
+template <typename T, int DP, bool VEC, bool SINK>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
+  constexpr int BQ = ATTN_BQ, ROWS = SINK ? SINK_TILE : BQ, LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32;
+  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD];
+  __shared__ __attribute__((aligned(16))) float sL[ROWS], sD[ROWS];
+  const int nk = SINK ? (a.S + 31) / 32 : (a.L + ATTN_BK - 1) / ATTN_BK, ns = SINK ? a.nsplit : 1;
+  long w = work_item((long)a.B * a.Hk * nk * ns);
+  if (w < 0) return;
+  const int tile = (int)(w % nk);
+  w /= nk;
+  const int split = (int)(w % ns);
+  w /= ns;
+  const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), G = a.H / a.Hk;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  const int len = row_length(a.lengths, b, a.L);
+  const int key0 = SINK ? tile * 32 : tile * ATTN_BK + wave * 32;  // the wave's 32 keys
+  const int sub = SINK ? wave * BQ : 0;                              // its queries inside the tile
+  long q_from, q_to;
+  if (SINK) {
+    const long rest = sink_rest(a.W), n = a.L > rest ? a.L - rest : 0;
+    const long per = ((n + ns - 1) / ns + ROWS - 1) / ROWS * ROWS;
+    q_from = rest + split * per;
+    q_to = q_from + per < len ? q_from + per : len;
+  } else {
+    const int k0 = tile * ATTN_BK;
+    q_from = k0 / BQ * BQ;
+    q_to = ((long)k0 + ATTN_BK - 1 + a.W - 1) / BQ * BQ + BQ;
+    q_to = q_to < len ? q_to : len;
+  }
+  const T *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
+  const float sc = a.scale * LOG2E;
+  Frag<T> kf[2][NC], vf[2][NC];
+  f32x4 dk[ND][2], dv[ND][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[d][i] = dv[d][i] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (len > 0) {
+      const int row = key0 + 16 * i + m;
+      const long r = min(row, len - 1);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        kf[i][c] = load8<T, VEC>(kp + r * a.k.t, c * 32 + g * 8, a.D);
+        vf[i][c] = load8<T, VEC>(vp + r * a.v.t, c * 32 + g * 8, a.D);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        kf[i][c] = zero_unless(kf[i][c], row < len, c * 32 + g * 8, a.D);
+        vf[i][c] = zero_unless(vf[i][c], row < len, c * 32 + g * 8, a.D);
+      }
+    }
+  }
+  const int per_head = q_to > q_from ? (int)((q_to - q_from + ROWS - 1) / ROWS) : 0, total = per_head * G;
+  Tile<T, ROWS, DP, 256, VEC> tq, tg;
+  float rl = INF, rd = 0.0f;
+  auto fetch = [&](int it) {
+    const int h = hk * G + it / per_head;
+    const long qi = q_from + (long)(it % per_head) * ROWS;
+    tq.load(head<T>(a.q, b, h), a.q.t, qi, len, a.D, tid);
+    tg.load(head<T>(a.dout, b, h), a.dout.t, qi, len, a.D, tid);
+    if (tid < ROWS) {
+      const long r = ((long)b * a.H + h) * a.L + (qi + tid < len ? qi + tid : len - 1);
+      rl = a.lse[r];
+      rd = a.delta[r];
+    }
+  };
+  if (total) fetch(0);
+  for (int it = 0; it < total; ++it) {
+    const long qi = q_from + (long)(it % per_head) * ROWS;
+    __syncthreads();
+    tq.store(sQ, qi, len, a.D, tid);
+    tg.store(sG, qi, len, a.D, tid);
+    if (tid < ROWS) {
+      sL[tid] = qi + tid < len ? rl : INF;
+      sD[tid] = qi + tid < len ? rd : 0.0f;
+    }
+    __syncthreads();
+    if (it + 1 < total) fetch(it + 1);
+    const int i0 = (int)qi + sub;
+    const int view = i0 < len && key0 < len ? tile_view(i0, i0 + BQ - 1, key0, key0 + 31, a.W, a.S) : 0;
+    if (!view) continue;
+    f32x4 s[2][2], dp[2][2];  // [query block][key block]: a lane holds four queries of one key
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) s[x][y] = dp[x][y] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const Frag<T> qf = along<T, DP>(sQ, sub + 16 * x, 32 * c, lane), gf = along<T, DP>(sG, sub + 16 * x, 32 * c, lane);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          mma(qf, kf[y][c], s[x][y]);
+          mma(gf, vf[y][c], dp[x][y]);
+        }
+      }
+    }
+    Frag<T> pf[2], df[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const f32x4 ls = *reinterpret_cast<const f32x4 *>(&sL[sub + 16 * x + 4 * g]);
+      const f32x4 de = *reinterpret_cast<const f32x4 *>(&sD[sub + 16 * x + 4 * g]);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p = exp2_fast(fmaf(s[x][y][r], sc, -ls[r]));
+          if (view == 1) p = sees(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? p : 0.0f;
+          const float d = p * (dp[x][y][r] - de[r]);
+          s[x][y][r] = p;
+          dp[x][y][r] = d;
+        }
+    }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      pf[y] = to_frag<T>(s[0][y], s[1][y]);
+      df[y] = to_frag<T>(dp[0][y], dp[1][y]);
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const Frag<T> gt = across<T, DP>(sG, sub, 16 * d, lane), qt = across<T, DP>(sQ, sub, 16 * d, lane);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        mma(gt, pf[y], dv[d][y]);
+        mma(qt, df[y], dk[d][y]);
+      }
+    }
+  }
+  const bool parts = a.nsplit > 0;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const int key = key0 + 16 * y + m;
+    if (SINK || (parts && key < a.S)) {
+      if (key < a.S) {
+        const long slot = SINK ? 1 + 4 * split + wave : 0;
+        float *p = a.part + ((((slot * a.B + b) * a.Hk + hk) * a.S + key) * 2) * a.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * d + 4 * g + r < a.D) {
+              p[16 * d + 4 * g + r] = dk[d][y][r] * a.scale;
+              p[a.D + 16 * d + 4 * g + r] = dv[d][y][r];
+            }
+      }
+    } else if (key < a.L) {
+      const long at0 = (((long)b * a.L + key) * a.Hk + hk) * a.D;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = dk[d][y][r] * a.scale;
+        store4<T, VEC>((T *)a.dk + at0, 16 * d + 4 * g, a.D, v);
+        store4<T, VEC>((T *)a.dv + at0, 16 * d + 4 * g, a.D, dv[d][y]);
+      }
+    }
+  }
+}
+
+// ---- the sinks' gradients from their parts
+template <typename T>
+__global__ __launch_bounds__(256) void bk_attn_sink_join_kernel(AttnArgs a) {
+  const int rows = a.S < a.L ? a.S : a.L;
+  const long per = (long)a.B * a.Hk * a.S * 2 * a.D, id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= per) return;
+  const int d = (int)(id % a.D), which = (int)(id / a.D % 2), key = (int)(id / (2 * a.D) % a.S);
+  const long bh = id / (2 * a.D) / a.S;
+  if (key >= rows) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int p = 0; p < 1 + 4 * a.nsplit; ++p) s += a.part[p * per + id];
+  const int b = (int)(bh / a.Hk), hk = (int)(bh % a.Hk);
+  ((T *)(which ? a.dv : a.dk))[(((long)b * a.L + key) * a.Hk + hk) * a.D + d] = (T)s;
+}
+
+// ---- one token: 4 waves over a stretch of the visible positions, 32 at a time each; up to 16 query heads of a key head
+// are the columns of one product.  The new token's key and value come from the call's operands and are written to the
+// cache by the first stretch; the slot they go to holds a position that is out of the window, so nobody reads it.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(256) void bk_attn_step_kernel(StepArgs a) {
+  constexpr int LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32, NV = 32 * (DP / 8) / 64;
+  constexpr int OUT = 4 * 16 * (DP + 4), TILE_BYTES = 4 * 32 * LD * (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char mem[TILE_BYTES > OUT * 4 ? TILE_BYTES : OUT * 4];
+  __shared__ float sM[4][16], sS[4][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+  unsigned w = blockIdx.x;
+  const int split = w % a.nsplit;
+  w /= a.nsplit;
+  const int hc = w % a.hchunks;
+  w /= a.hchunks;
+  const int hk = w % a.Hk, b = w / a.Hk, G = a.H / a.Hk;
+  const int pos = a.positions[b];
+  const int nh = min(16, G - hc * 16), h0 = hk * G + hc * 16;
+  const T *kc = head<T>(a.kc, b, hk), *vc = head<T>(a.vc, b, hk);
+  const T *kn = head<T>(a.k, b, hk), *vn = head<T>(a.v, b, hk);
+  const int ring = a.cap - a.S;
+  const int first = max(a.S, pos - a.W + 1);                     // first position of the window behind the sinks
+  const int nsink = pos < 0 ? 0 : min(a.S, pos + 1), n = pos < 0 ? 0 : nsink + max(0, pos - first + 1);
+  auto slot = [&](int t) {  // of the t-th visible position
+    return t < nsink ? t : a.S + (first - a.S + t - nsink) % ring;
+  };
+  if (pos >= 0 && split == 0 && hc == 0) {
+    const long at0 = pos < a.S ? pos : a.S + (pos - a.S) % ring;
+    T *ko = const_cast<T *>(kc) + at0 * a.kc.t, *vo = const_cast<T *>(vc) + at0 * a.vc.t;
+    for (int d = tid; d < a.D; d += 256) {
+      ko[d] = kn[d];
+      vo[d] = vn[d];
+    }
+  }
+  Frag<T> q[NC];
+  {
+    const T *qp = head<T>(a.q, b, h0 + min(m, nh - 1));
+#pragma unroll
+    for (int c = 0; c < NC; ++c) q[c] = load8<T, VEC>(qp, c * 32 + g * 8, a.D);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) q[c] = zero_unless(q[c], m < nh, c * 32 + g * 8, a.D);
+  }
+  f32x4 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float mx = -INF, sum = 0.0f;
+  const float sc = a.scale * LOG2E;
+  const int from = split * a.per, to = min(n, from + a.per);
+  T *sV = (T *)mem + wave * 32 * LD;
+  Frag<T> kr[2][NC], vr[NV];
+  auto row = [&](const T *cache, const T *fresh, long stride, int t) {  // the newest position is not in the cache yet
+    return t >= n - 1 ? fresh : cache + (long)slot(t) * stride;
+  };
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const T *p = row(kc, kn, a.kc.t, t0 + 16 * k + m);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) kr[k][c] = load8<T, VEC>(p, c * 32 + g * 8, a.D);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = lane + 64 * k;
+      vr[k] = load8<T, VEC>(row(vc, vn, a.vc.t, t0 + i / (DP / 8)), (i % (DP / 8)) * 8, a.D);
+    }
+  };
+  if (from + wave * 32 < to) fetch(from + wave * 32);
+  for (int t0 = from + wave * 32; t0 < to; t0 += 128) {
+    f32x4 s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      s[k] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (!VEC || a.D < DP) kr[k][c] = zero_unless(kr[k][c], true, c * 32 + g * 8, a.D);
+        mma(kr[k][c], q[c], s[k]);
+      }
+    }
+    // the wave's own LDS rows: its accesses stay in order, no other wave touches them
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = lane + 64 * k, r = i / (DP / 8), c = (i % (DP / 8)) * 8;
+      const Frag<T> f = zero_unless(vr[k], t0 + r < to, c, a.D);
+      *reinterpret_cast<typename Frag<T>::vec *>(sV + r * LD + c) = f.v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (t0 + 128 < to) fetch(t0 + 128);
+    float top = -INF;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[k][r] = t0 + 16 * k + 4 * g + r < to ? s[k][r] * sc : -INF;
+        top = fmaxf(top, s[k][r]);
+      }
+    top = fmaxf(mx, col_max(top));
+    const float ref = top == -INF ? 0.0f : top, alpha = exp2_fast(mx - ref);
+    mx = top;
+    float part = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[k][r] = exp2_fast(s[k][r] - ref);
+        part += s[k][r];
+      }
+    sum = fmaf(sum, alpha, part);
+    const Frag<T> p = to_frag<T>(s[0], s[1]);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
+      mma(across<T, DP>(sV, 0, 16 * d, lane), p, o[d]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  sum = col_sum(sum);
+  __syncthreads();  // the value rows are done with: their memory takes the waves' results
+  float *sO = (float *)mem;
+  if (g == 0) {
+    sM[wave][m] = mx;
+    sS[wave][m] = sum;
+  }
+#pragma unroll
+  for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&sO[(wave * 16 + m) * (DP + 4) + 16 * d + 4 * g]) = o[d];
+  __syncthreads();
+  for (int i = tid; i < nh * a.D; i += 256) {
+    const int h = i / a.D, d = i % a.D;
+    float top = -INF, l = 0.0f, acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, sM[k][h]);
+    const float ref = top == -INF ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = exp2_fast(sM[k][h] - ref);
+      l = fmaf(sS[k][h], f, l);
+      acc = fmaf(sO[(k * 16 + h) * (DP + 4) + d], f, acc);
+    }
+    const long bh = (long)b * a.H + h0 + h;
+    if (a.nsplit == 1) {
+      ((T *)a.o)[bh * a.D + d] = (T)(l > 0.0f || l != l ? acc / l : 0.0f);
+    } else {
+      float *p = a.part + ((long)split * a.B * a.H + bh) * (a.D + 2);
+      p[d] = acc;
+      if (d == 0) {
+        p[a.D] = top;
+        p[a.D + 1] = l;
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(128) void bk_attn_step_join_kernel(StepArgs a) {
+  const long bh = blockIdx.x, stride = (long)a.B * a.H * (a.D + 2);
+  const float *p = a.part + bh * (a.D + 2);
+  float top = -INF;
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, p[s * stride + a.D]);
+  const float ref = top == -INF ? 0.0f : top;
+  const int d = threadIdx.x;
+  if (d >= a.D) return;
+  float l = 0.0f, acc = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float f = exp2_fast(p[s * stride + a.D] - ref);
+    l = fmaf(p[s * stride + a.D + 1], f, l);
+    acc = fmaf(p[s * stride + d], f, acc);
+  }
+  ((T *)a.o)[bh * a.D + d] = (T)(l > 0.0f || l != l ? acc / l : 0.0f);
+}
+
+}  // namespace
+
+#define BK_ATTN_DP(LAUNCH)                                            \
+  do {                                                                \
+    if (dp == 32) { if (vec) LAUNCH(32, true); else LAUNCH(32, false); }        \
+    else if (dp == 64) { if (vec) LAUNCH(64, true); else LAUNCH(64, false); }   \
+    else { if (vec) LAUNCH(128, true); else LAUNCH(128, false); }     \
+  } while (0)
+
+template <typename T>
+void attn_forward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
+  const unsigned grid = work_grid((long)a.B * a.H * ((a.L + ATTN_BM - 1) / ATTN_BM));
+#define BK_LAUNCH(DP, VEC) hipLaunchKernelGGL((bk_attn_kernel<T, DP, VEC>), dim3(grid), dim3(256), 0, s, a)
+  BK_ATTN_DP(BK_LAUNCH);
+#undef BK_LAUNCH
+}
+
+template <typename T>
+void attn_backward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
+  const long rows = (long)a.B * a.H * a.L;
+  hipLaunchKernelGGL((bk_attn_delta_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  const unsigned grid_q = work_grid((long)a.B * a.H * ((a.L + ATTN_BM - 1) / ATTN_BM));
+  const unsigned grid_k = work_grid((long)a.B * a.Hk * ((a.L + ATTN_BK - 1) / ATTN_BK));
+  const unsigned grid_s = work_grid((long)a.B * a.Hk * ((a.S + 31) / 32) * a.nsplit);
+#define BK_LAUNCH(DP, VEC)                                                                                      \
+  do {                                                                                                          \
+    hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, false>), dim3(grid_k), dim3(256), 0, s, a);              \
+    if (a.nsplit) hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, true>), dim3(grid_s), dim3(256), 0, s, a); \
+    hipLaunchKernelGGL((bk_attn_dq_kernel<T, DP, VEC>), dim3(grid_q), dim3(256), 0, s, a);                      \
+  } while (0)
+  BK_ATTN_DP(BK_LAUNCH);
+#undef BK_LAUNCH
+  if (a.nsplit) {
+    const long per = (long)a.B * a.Hk * a.S * 2 * a.D;
+    hipLaunchKernelGGL((bk_attn_sink_join_kernel<T>), dim3((unsigned)((per + 255) / 256)), dim3(256), 0, s, a);
+  }
+}
+
+template <typename T>
+void attn_step(const StepArgs &a, int dp, bool vec, hipStream_t s) {
+  const unsigned grid = (unsigned)(a.B * a.Hk * a.hchunks * a.nsplit);
+#define BK_LAUNCH(DP, VEC) hipLaunchKernelGGL((bk_attn_step_kernel<T, DP, VEC>), dim3(grid), dim3(256), 0, s, a)
+  BK_ATTN_DP(BK_LAUNCH);
+#undef BK_LAUNCH
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((bk_attn_step_join_kernel<T>), dim3((unsigned)(a.B * a.H)), dim3(128), 0, s, a);
+}
+
+}  // namespace bk

@@ -207,3 +207,55 @@ def directional(f, args, grads, index, seed, step=1e-6):
     fd = float((f(*plus) - f(*minus)) / (2 * step))
     gd = d64(grads[index])
     return float((gd * v).sum()), fd, float((gd * v).abs().sum())
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+
+def attention(q, k, v, window, sinks, scale, u, lens=None, do=None):
+    """dict of values (o and with do: dq, dk, dv) and bounds (e + name); u is half a step of the operands' type.
+
+    Scores: D products in float32, 2 D u32 of sum |q_i k_j|, plus the base-2 exponential (4 u32 and the scaled score's own
+    rounding): ep is what that is worth relative to a probability.  Probabilities and score gradients are rounded to the
+    operands' type before the second products (u each, and 2^-25 below float16's normal range); sums over up to L keys in
+    float32 add L u32 at most."""
+    B, H, L, D = q.shape
+    Hk = k.shape[1]
+    G = H // Hk
+    lens = [L] * B if lens is None else [min(max(int(n), 0), L) for n in lens]
+    r = {n: torch.zeros_like(q) for n in ("o", "eo", "dq", "edq")}
+    r.update({n: torch.zeros_like(k) for n in ("dk", "edk", "dv", "edv")})
+    tiny = 2.0 ** -25 if u == half_step(torch.float16) else 0.0
+    ur = 0.0 if u == half_step(torch.float32) else u
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+        see = (j <= i) & ((i - j < window) | (j < sinks))
+        for h in range(H):
+            Q, K, V = q[b, h, :n], k[b, h // G, :n], v[b, h // G, :n]
+            s = (Q @ K.t()) * scale
+            mag = (Q.abs() @ K.t().abs()) * abs(scale)
+            p = torch.softmax(s.masked_fill(~see, -math.inf), -1)
+            ep = (2 * D * U32 * mag + 8 * U32 * (1 + mag)).masked_fill(~see, 0)
+            ep = ep + (p * ep).sum(-1, keepdim=True) + (n + 20) * U32        # the score's own error, the sum's, its rounding
+            o = p @ V
+            pe = p * (ep + ur) + tiny * see
+            r["o"][b, h, :n] = o
+            r["eo"][b, h, :n] = pe @ V.abs() + (n + 10) * U32 * (p @ V.abs())
+            if do is None:
+                continue
+            g = do[b, h, :n]
+            dp, Dp = g @ V.t(), g.abs() @ V.abs().t()
+            # delta comes from the output as it was stored
+            eo = r["eo"][b, h, :n] + ur * o.abs()
+            delta, ede = (g * o).sum(-1, keepdim=True), (g.abs() * (eo + (D + 4) * U32 * o.abs())).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            eds = p * ((ep + 2 * U32) * (dp - delta).abs() + 2 * D * U32 * Dp + ede) + ur * ds.abs() + tiny * see
+            more = (n * G + 20) * U32
+            r["dq"][b, h, :n] = ds @ K * scale
+            r["edq"][b, h, :n] = (eds + more * ds.abs()) @ K.abs() * abs(scale)
+            r["dk"][b, h // G, :n] += ds.t() @ Q * scale
+            r["edk"][b, h // G, :n] += (eds + more * ds.abs()).t() @ Q.abs() * abs(scale)
+            r["dv"][b, h // G, :n] += p.t() @ g
+            r["edv"][b, h // G, :n] += (pe + more * p).t() @ g.abs()
+    return r

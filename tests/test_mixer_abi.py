@@ -73,3 +73,33 @@ def test_operators_refuse_cpu_tensors():
                  lambda: bkcore.selective_scan(x, x, torch.zeros(8, 4), x[..., :4], x[..., :4])):
         with pytest.raises(RuntimeError, match="ROCm device"):
             call()
+
+
+def test_sliding_attention(L):
+    def fwd(dt=1, B=1, H=4, Hk=2, T=8, D=16, W=4, S=1, scale=0.25, q=p, out=p):
+        return L.bkcore_sliding_attention(q, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, dt, None, B, H, Hk, T, D, W, S, scale, out, None,
+                                          None)
+    assert fwd(B=0) == OK and fwd(T=0) == OK
+    for bad in (dict(dt=3), dict(H=3), dict(Hk=0), dict(D=0), dict(D=129), dict(W=0), dict(S=-1), dict(S=65),
+                dict(scale=float("nan")), dict(B=-1), dict(q=None), dict(out=None)):
+        assert fwd(**bad) == EINVAL, bad
+
+    def bwd(ws, n, T=2000, lse=p):
+        return L.bkcore_sliding_attention_backward(p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, lse, 1, None, 1, 4, 2, T, 16,
+                                                   8, 2, 0.25, p, p, p, ws, n, None)
+    need = L.bkcore_sliding_attention_backward_workspace_bytes(1, 4, 2, 2000, 16, 8, 2)
+    assert need > 4 * 2000 * 4                              # delta, and the sinks' partial sums of a long rest
+    assert L.bkcore_sliding_attention_backward_workspace_bytes(1, 4, 2, 2000, 16, 8, 0) == 4 * 2000 * 4
+    assert bwd(None, 0) == EWS and bwd(p, need - 1) == EWS and bwd(p, need, lse=None) == EINVAL
+
+    def step(cap=10, W=8, S=2, ws=None, n=0, pos=p):
+        return L.bkcore_sliding_attention_step(p, 1, 1, p, 1, 1, p, 1, 1, p, 1, 1, 16, p, 1, 1, 16, pos, 1, 1, 4, 2, cap, 16, W, S,
+                                               0.25, p, ws, n, None)
+    assert step(cap=9) == EINVAL and step(pos=None) == EINVAL and step(W=0) == EINVAL
+    need = L.bkcore_sliding_attention_step_workspace_bytes(1, 4, 2, 5000, 16, 4096, 4)
+    assert need > 0 and step(cap=5000, W=4096, S=4) == EWS and step(cap=5000, W=4096, S=4, ws=p, n=need - 1) == EWS
+    assert L.bkcore_sliding_attention_step_workspace_bytes(1, 4, 2, 10, 16, 8, 2) == 0
+
+    def fill(cap=10, S=2, D=16, k=p):
+        return L.bkcore_sliding_cache_fill(k, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 16, p, 1, 1, 16, None, 1, 1, 2, 8, cap, D, S, None)
+    assert fill(cap=2) == EINVAL and fill(D=129) == EINVAL and fill(k=None) == EINVAL
