@@ -432,21 +432,22 @@ int bkcore_selective_scan_step(const void *x, int64_t x_batch, float *state, con
  * j < sinks (the first tokens, at most 64), H query heads over Hk key / value heads (H a multiple of Hk; neighbouring query
  * heads share one).  Takes the place of the windowed local path (src/models/phase7/hybrid_attention.py:93-103), whose
  * windows are blocks.  q (B, H, L, D), k, v (B, Hk, L, D) by strides, D <= 128; out (B, L, H, D) contiguous; lse: NULL, or
- * (B, H, L) floats for the backward (base-2 logarithm of the row's sum; +inf for a row that sees nothing). */
+ * (B, H, L) floats for the backward (base-2 logarithm of the row's sum; +inf for a row that sees nothing); out_lo: NULL, or
+ * what rounding took from out (out's layout and type), which the backward adds back where the output enters it. */
 #define BKCORE_ATTENTION_MAX_HEAD_DIM 128
 #define BKCORE_ATTENTION_MAX_SINKS 64
 int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t q_head, int64_t q_time, const void *k,
                              int64_t k_batch, int64_t k_head, int64_t k_time, const void *v, int64_t v_batch,
                              int64_t v_head, int64_t v_time, int dtype, const int *lengths, int64_t B, int64_t H, int64_t Hk,
-                             int64_t L, int64_t D, int64_t window, int64_t sinks, float scale, void *out, float *lse,
-                             void *stream);
+                             int64_t L, int64_t D, int64_t window, int64_t sinks, float scale, void *out, void *out_lo,
+                             float *lse, void *stream);
 /* dq (B, L, H, D), dk, dv (B, L, Hk, D) contiguous; sums in a fixed order (no atomics). */
 size_t bkcore_sliding_attention_backward_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D,
                                                          int64_t window, int64_t sinks);
 int bkcore_sliding_attention_backward(const void *dout, int64_t do_batch, int64_t do_head, int64_t do_time, const void *q,
                                       int64_t q_batch, int64_t q_head, int64_t q_time, const void *k, int64_t k_batch,
                                       int64_t k_head, int64_t k_time, const void *v, int64_t v_batch, int64_t v_head,
-                                      int64_t v_time, const void *out, const float *lse, int dtype, const int *lengths,
+                                      int64_t v_time, const void *out, const void *out_lo, const float *lse, int dtype, const int *lengths,
                                       int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D, int64_t window, int64_t sinks,
                                       float scale, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
                                       void *stream);

@@ -152,8 +152,8 @@ def _declare(L):
                                         sz, vp],
             "selective_scan_step": [vp, i64, vp, vp, i64, vp, vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i64, i64, i64, vp,
                                     vp],
-            "sliding_attention": [vp, i64, i64, i64] * 3 + [i32, vp] + [i64] * 7 + [f32, vp, vp, vp],
-            "sliding_attention_backward": [vp, i64, i64, i64] * 4 + [vp, vp, i32, vp] + [i64] * 7 + [f32, vp, vp, vp, vp, sz,
+            "sliding_attention": [vp, i64, i64, i64] * 3 + [i32, vp] + [i64] * 7 + [f32, vp, vp, vp, vp],
+            "sliding_attention_backward": [vp, i64, i64, i64] * 4 + [vp, vp, vp, i32, vp] + [i64] * 7 + [f32, vp, vp, vp, vp, sz,
                                                                                                   vp],
             "sliding_attention_step": [vp, i64, i64] * 3 + [vp, i64, i64, i64] * 2 + [vp, i32] + [i64] * 7 + [f32, vp, vp, sz,
                                                                                                             vp],

@@ -53,22 +53,23 @@ class _SlidingAttentionFunction(torch.autograd.Function):
         dev = q.device
         o = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
         lse = torch.empty(B * H * T, dtype=torch.float32, device=dev) if keep else None
+        lo = torch.empty_like(o) if keep and q.dtype != torch.float32 else None   # what rounding takes from the output
         with ops.on_device(dev):
             rc = _lib.load_held().bkcore_sliding_attention(
                 q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-                ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window, sinks, scale, o.data_ptr(), ops.ptr(lse),
+                ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window, sinks, scale, o.data_ptr(), ops.ptr(lo), ops.ptr(lse),
                 ops.stream(dev.index))
         if rc:
             _lib.check(rc, "bkcore_sliding_attention")
         if keep:
-            ctx.save_for_backward(q, k, v, o, lse, lengths)
+            ctx.save_for_backward(q, k, v, o, lo, lse, lengths)
             ctx.bk_args = window, sinks, scale
         return o.transpose(1, 2)
 
     @staticmethod
     def backward(ctx, do):
         ops.once_only("sliding_attention")
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, lo, lse, lengths = ctx.saved_tensors
         window, sinks, scale = ctx.bk_args
         do = ops.inner(do)
         B, H, T, D = q.shape
@@ -83,7 +84,7 @@ class _SlidingAttentionFunction(torch.autograd.Function):
         with ops.on_device(dev):
             rc = L.bkcore_sliding_attention_backward(
                 do.data_ptr(), *do.stride()[:3], q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(),
-                *v.stride()[:3], o.data_ptr(), lse.data_ptr(), ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window,
+                *v.stride()[:3], o.data_ptr(), ops.ptr(lo), lse.data_ptr(), ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window,
                 sinks, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes, ops.stream(dev.index))
         if rc:
             _lib.check(rc, "bkcore_sliding_attention_backward")

@@ -16,6 +16,7 @@ struct AttnArgs {
   Heads q, k, v, dout;
   const void *out;          // forward's output for the backward, (B, L, H, D) contiguous like o, dq, dk, dv
   void *o, *dq, *dk, *dv;
+  void *lo;                 // what rounding took from the output, for delta (16-bit operands; may be null)
   float *lse, *delta, *part;  // log2 of the row's sum, (B, H, L); rows that see nothing hold +inf
   const int *lengths;
   int B, H, Hk, L, D, W, S;

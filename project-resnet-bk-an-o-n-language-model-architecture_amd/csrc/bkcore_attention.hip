@@ -66,7 +66,7 @@ extern "C" int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t 
                                         int64_t k_batch, int64_t k_head, int64_t k_time, const void *v, int64_t v_batch,
                                         int64_t v_head, int64_t v_time, int dtype, const int *lengths, int64_t B, int64_t H,
                                         int64_t Hk, int64_t L, int64_t D, int64_t window, int64_t sinks, float scale,
-                                        void *out, float *lse, void *stream) {
+                                        void *out, void *out_lo, float *lse, void *stream) {
   const int rc = check(dtype, B, H, Hk, L, D, window, sinks, scale);
   if (rc) return rc;
   if (B == 0 || L == 0) return BKCORE_OK;
@@ -76,11 +76,11 @@ extern "C" int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t 
   a.q = {q, q_batch, q_head, q_time};
   a.k = {k, k_batch, k_head, k_time};
   a.v = {v, v_batch, v_head, v_time};
-  a.o = out; a.lse = lse; a.lengths = lengths;
+  a.o = out; a.lo = out_lo; a.lse = lse; a.lengths = lengths;
   a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.L = (int)L; a.D = (int)D; a.S = (int)(sinks < L ? sinks : L);
   a.W = (int)(window < L ? window : L); a.scale = scale;
   const bool vec = D % 8 == 0 && rows_aligned(a.q, dtype) && rows_aligned(a.k, dtype) && rows_aligned(a.v, dtype) &&
-                   aligned16(out);
+                   aligned16(out) && aligned16(out_lo);
   BK_WITH_TYPE(dtype, attn_forward<T>(a, padded(D), vec, (hipStream_t)stream));
   return launch_status();
 }
@@ -97,14 +97,14 @@ extern "C" size_t bkcore_sliding_attention_backward_workspace_bytes(int64_t B, i
 extern "C" int bkcore_sliding_attention_backward(
     const void *dout, int64_t do_batch, int64_t do_head, int64_t do_time, const void *q, int64_t q_batch, int64_t q_head,
     int64_t q_time, const void *k, int64_t k_batch, int64_t k_head, int64_t k_time, const void *v, int64_t v_batch,
-    int64_t v_head, int64_t v_time, const void *out, const float *lse, int dtype, const int *lengths, int64_t B, int64_t H,
+    int64_t v_head, int64_t v_time, const void *out, const void *out_lo, const float *lse, int dtype, const int *lengths, int64_t B, int64_t H,
     int64_t Hk, int64_t L, int64_t D, int64_t window, int64_t sinks, float scale, void *dq, void *dk, void *dv,
     void *workspace, size_t workspace_bytes, void *stream) {
   const int rc = check(dtype, B, H, Hk, L, D, window, sinks, scale);
   if (rc) return rc;
   if (B == 0 || L == 0) return BKCORE_OK;
   if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return BKCORE_EINVAL;
-  if (B * H * L > 4LL * 2147483000LL) return BKCORE_EINVAL;
+  if (B * H * L > 2147483000LL * 16) return BKCORE_EINVAL;
   if (!workspace || workspace_bytes < bkcore_sliding_attention_backward_workspace_bytes(B, H, Hk, L, D, window, sinks))
     return BKCORE_EWORKSPACE;
   AttnArgs a{};
@@ -112,14 +112,14 @@ extern "C" int bkcore_sliding_attention_backward(
   a.q = {q, q_batch, q_head, q_time};
   a.k = {k, k_batch, k_head, k_time};
   a.v = {v, v_batch, v_head, v_time};
-  a.out = out; a.lse = const_cast<float *>(lse); a.lengths = lengths; a.dq = dq; a.dk = dk; a.dv = dv;
+  a.out = out; a.lo = const_cast<void *>(out_lo); a.lse = const_cast<float *>(lse); a.lengths = lengths; a.dq = dq; a.dk = dk; a.dv = dv;
   a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.L = (int)L; a.D = (int)D; a.S = (int)(sinks < L ? sinks : L);
   a.W = (int)(window < L ? window : L); a.scale = scale;
   a.nsplit = sink_splits(B, Hk, L, a.W, a.S);
   a.delta = (float *)workspace;
   a.part = a.delta + (((size_t)B * H * L + 3) & ~(size_t)3);
   const bool vec = D % 8 == 0 && rows_aligned(a.q, dtype) && rows_aligned(a.k, dtype) && rows_aligned(a.v, dtype) &&
-                   rows_aligned(a.dout, dtype) && aligned16(dq) && aligned16(dk) && aligned16(dv);
+                   rows_aligned(a.dout, dtype) && aligned16(out) && aligned16(out_lo) && aligned16(dq) && aligned16(dk) && aligned16(dv);
   BK_WITH_TYPE(dtype, attn_backward<T>(a, padded(D), vec, (hipStream_t)stream));
   return launch_status();
 }

@@ -206,7 +206,7 @@ __device__ __forceinline__ bool sees(int i, int j, int W, int S) { return j <= i
 
 // ---- forward: 4 waves x 32 queries; keys and values through LDS, the next tile on its way in registers.
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256) void bk_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
   constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32;
   __shared__ __attribute__((aligned(16))) T sK[BN * LD], sV[BN * LD];
   const int nq = (a.L + ATTN_BM - 1) / ATTN_BM;
@@ -330,6 +330,12 @@ __global__ __launch_bounds__(256) void bk_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = row < len ? o[d][i][r] * inv : 0.0f;
         store4<T, VEC>(op, 16 * d + 4 * g, a.D, v);
+        if (a.lo) {
+          f32x4 e;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) e[r] = v[r] - (float)(T)v[r];
+          store4<T, VEC>((T *)a.lo + (op - (T *)a.o), 16 * d + 4 * g, a.D, e);
+        }
       }
       if (a.lse && g == 0)
         a.lse[((long)b * a.H + h) * a.L + row] =
@@ -338,27 +344,38 @@ __global__ __launch_bounds__(256) void bk_attn_kernel(AttnArgs a) {
   }
 }
 
-// ---- delta_i = do_i . o_i, one wave a row
-template <typename T>
+// ---- delta_i = do_i . o_i: a row's D elements over TPR = DP / 8 lanes.  A 16-bit output's rounding is added back (lo):
+// it would reach every score gradient of the row.
+template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(256) void bk_attn_delta_kernel(AttnArgs a) {
-  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (id >= (long)a.B * a.L * a.H) return;
-  const int h = (int)(id % a.H);
-  const long bt = id / a.H;
+  constexpr int TPR = DP / 8;
+  const long id = ((long)blockIdx.x * 256 + threadIdx.x) / TPR;
+  const int c = (threadIdx.x % TPR) * 8;
+  const long total = (long)a.B * a.L * a.H;
+  const long i = id < total ? id : total - 1;
+  const int h = (int)(i % a.H);
+  const long bt = i / a.H;
   const int b = (int)(bt / a.L), t = (int)(bt % a.L);
+  const Frag<T> o = load8<T, VEC>((const T *)a.out + i * a.D, c, a.D);
+  const Frag<T> gr = load8<T, VEC>(head<T>(a.dout, b, h) + (long)t * a.dout.t, c, a.D);
+  Frag<T> lo;
+  if (a.lo) lo = load8<T, VEC>((const T *)a.lo + i * a.D, c, a.D);
   float s = 0.0f;
   if (t < row_length(a.lengths, b, a.L)) {
-    const T *o = (const T *)a.out + id * a.D, *g = head<T>(a.dout, b, h) + (long)t * a.dout.t;
-    for (int d = lane; d < a.D; d += 64) s = fmaf((float)o[d], (float)g[d], s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < a.D) s = fmaf((float)o.v[k] + (a.lo ? (float)lo.v[k] : 0.0f), (float)gr.v[k], s);
   }
-  s = wave_sum(s);
-  if (lane == 0) a.delta[((long)b * a.H + h) * a.L + t] = s;
+  s += dpp_mov<DPP_XOR1>(s);
+  s += dpp_mov<DPP_XOR2>(s);
+  if constexpr (TPR >= 8) s += dpp_mov<DPP_HALF_MIRROR>(s);
+  if constexpr (TPR >= 16) s += dpp_mov<DPP_MIRROR>(s);
+  if (id < total && c == 0) a.delta[((long)b * a.H + h) * a.L + t] = s;
 }
 
 // ---- dq: the forward's loop with two score products, dS^T in the lane, and K contracted over its rows.
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256) void bk_attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_kernel(AttnArgs a) {
   constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32;
   __shared__ __attribute__((aligned(16))) T sK[BN * LD], sV[BN * LD];
   const int nq = (a.L + ATTN_BM - 1) / ATTN_BM;
@@ -426,33 +443,29 @@ __global__ __launch_bounds__(256) void bk_attn_dq_kernel(AttnArgs a) {
     if (!view) continue;
 #pragma unroll
     for (int k = 0; k < NK; k += 2) {
-      f32x4 s[2][2], dp[2][2];
+      Frag<T> ds[2];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        s[kk][0] = s[kk][1] = dp[kk][0] = dp[kk][1] = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 s[2], dp[2];
+        s[0] = s[1] = dp[0] = dp[1] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const Frag<T> kf = along<T, DP>(sK, 16 * (k + kk), 32 * c, lane), vf = along<T, DP>(sV, 16 * (k + kk), 32 * c, lane);
-          mma(kf, q[0][c], s[kk][0]);
-          mma(kf, q[1][c], s[kk][1]);
-          mma(vf, go[0][c], dp[kk][0]);
-          mma(vf, go[1][c], dp[kk][1]);
+          mma(kf, q[0][c], s[0]);
+          mma(kf, q[1][c], s[1]);
+          mma(vf, go[0][c], dp[0]);
+          mma(vf, go[1][c], dp[1]);
         }
-      }
-      Frag<T> ds[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int qi = w0 + 16 * i + m;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int i = 0; i < 2; ++i) {
+          const int qi = w0 + 16 * i + m;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = exp2_fast(fmaf(s[kk][i][r], sc, -lse[i]));
-            float x = p * (dp[kk][i][r] - delta[i]);
+            float x = exp2_fast(fmaf(s[i][r], sc, -lse[i])) * (dp[i][r] - delta[i]);
             if (view == 1) x = sees(qi, j0 + 16 * (k + kk) + 4 * g + r, a.W, a.S) ? x : 0.0f;
-            s[kk][i][r] = x;
+            ds[i].v[4 * kk + r] = (T)x;
           }
-        ds[i] = to_frag<T>(s[0][i], s[1][i]);
+        }
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
@@ -484,7 +497,7 @@ __global__ __launch_bounds__(256) void bk_attn_dq_kernel(AttnArgs a) {
 // 32 of every 128 queries, and leaves float32 sums that the join adds up in a fixed order.
 // part: (1 + 4 nsplit, B, Hk, S, 2, D); slot 0 is what the first key tile has from its own queries.
 template <typename T, int DP, bool VEC, bool SINK>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
   constexpr int BQ = ATTN_BQ, ROWS = SINK ? SINK_TILE : BQ, LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32;
   __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD];
   __shared__ __attribute__((aligned(16))) float sL[ROWS], sD[ROWS];
@@ -564,41 +577,31 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void bk_attn_dkv_kernel(Att
     const int i0 = (int)qi + sub;
     const int view = i0 < len && key0 < len ? tile_view(i0, i0 + BQ - 1, key0, key0 + 31, a.W, a.S) : 0;
     if (!view) continue;
-    f32x4 s[2][2], dp[2][2];  // [query block][key block]: a lane holds four queries of one key
+    Frag<T> pf[2], df[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-#pragma unroll
-      for (int y = 0; y < 2; ++y) s[x][y] = dp[x][y] = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 s[2], dp[2];  // of the key blocks: a lane holds four queries of one key
+      s[0] = s[1] = dp[0] = dp[1] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const Frag<T> qf = along<T, DP>(sQ, sub + 16 * x, 32 * c, lane), gf = along<T, DP>(sG, sub + 16 * x, 32 * c, lane);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          mma(qf, kf[y][c], s[x][y]);
-          mma(gf, vf[y][c], dp[x][y]);
+          mma(qf, kf[y][c], s[y]);
+          mma(gf, vf[y][c], dp[y]);
         }
       }
-    }
-    Frag<T> pf[2], df[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
       const f32x4 ls = *reinterpret_cast<const f32x4 *>(&sL[sub + 16 * x + 4 * g]);
       const f32x4 de = *reinterpret_cast<const f32x4 *>(&sD[sub + 16 * x + 4 * g]);
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float p = exp2_fast(fmaf(s[x][y][r], sc, -ls[r]));
+          float p = exp2_fast(fmaf(s[y][r], sc, -ls[r]));
           if (view == 1) p = sees(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? p : 0.0f;
-          const float d = p * (dp[x][y][r] - de[r]);
-          s[x][y][r] = p;
-          dp[x][y][r] = d;
+          pf[y].v[4 * x + r] = (T)p;
+          df[y].v[4 * x + r] = (T)(p * (dp[y][r] - de[r]));
         }
-    }
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      pf[y] = to_frag<T>(s[0][y], s[1][y]);
-      df[y] = to_frag<T>(dp[0][y], dp[1][y]);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
@@ -849,12 +852,13 @@ void attn_forward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
 template <typename T>
 void attn_backward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
   const long rows = (long)a.B * a.H * a.L;
-  hipLaunchKernelGGL((bk_attn_delta_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  const unsigned grid_d = (unsigned)((rows * (dp / 8) + 255) / 256);
   const unsigned grid_q = work_grid((long)a.B * a.H * ((a.L + ATTN_BM - 1) / ATTN_BM));
   const unsigned grid_k = work_grid((long)a.B * a.Hk * ((a.L + ATTN_BK - 1) / ATTN_BK));
   const unsigned grid_s = work_grid((long)a.B * a.Hk * ((a.S + 31) / 32) * a.nsplit);
 #define BK_LAUNCH(DP, VEC)                                                                                      \
   do {                                                                                                          \
+    hipLaunchKernelGGL((bk_attn_delta_kernel<T, DP, VEC>), dim3(grid_d), dim3(256), 0, s, a);                   \
     hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, false>), dim3(grid_k), dim3(256), 0, s, a);              \
     if (a.nsplit) hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, true>), dim3(grid_s), dim3(256), 0, s, a); \
     hipLaunchKernelGGL((bk_attn_dq_kernel<T, DP, VEC>), dim3(grid_q), dim3(256), 0, s, a);                      \

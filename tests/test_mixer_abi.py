@@ -77,7 +77,7 @@ def test_operators_refuse_cpu_tensors():
 
 def test_sliding_attention(L):
     def fwd(dt=1, B=1, H=4, Hk=2, T=8, D=16, W=4, S=1, scale=0.25, q=p, out=p):
-        return L.bkcore_sliding_attention(q, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, dt, None, B, H, Hk, T, D, W, S, scale, out, None,
+        return L.bkcore_sliding_attention(q, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, dt, None, B, H, Hk, T, D, W, S, scale, out, None, None,
                                           None)
     assert fwd(B=0) == OK and fwd(T=0) == OK
     for bad in (dict(dt=3), dict(H=3), dict(Hk=0), dict(D=0), dict(D=129), dict(W=0), dict(S=-1), dict(S=65),
@@ -85,7 +85,7 @@ def test_sliding_attention(L):
         assert fwd(**bad) == EINVAL, bad
 
     def bwd(ws, n, T=2000, lse=p):
-        return L.bkcore_sliding_attention_backward(p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, lse, 1, None, 1, 4, 2, T, 16,
+        return L.bkcore_sliding_attention_backward(p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, None, lse, 1, None, 1, 4, 2, T, 16,
                                                    8, 2, 0.25, p, p, p, ws, n, None)
     need = L.bkcore_sliding_attention_backward_workspace_bytes(1, 4, 2, 2000, 16, 8, 2)
     assert need > 4 * 2000 * 4                              # delta, and the sinks' partial sums of a long rest
