@@ -54,9 +54,13 @@ def no_grad_through(what: str, *tensors) -> None:
         raise RuntimeError(f"bkcore: {what} serves single tokens and has no gradient; call it under torch.no_grad()")
 
 
+FAR = 1 << 24     # strides between positions from here on are beyond the kernels' 32-bit offsets inside a tile
+
+
 def inner(t: torch.Tensor | None) -> torch.Tensor | None:
-    """The tensor itself when its last dimension has unit stride, else a contiguous copy."""
-    if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1:
+    """The tensor itself when its last dimension has unit stride (and its positions lie near enough), else a contiguous
+    copy."""
+    if t is None or ((t.shape[-1] <= 1 or t.stride(-1) == 1) and (t.dim() < 2 or t.stride(-2) < FAR)):
         return t
     return t.contiguous()
 

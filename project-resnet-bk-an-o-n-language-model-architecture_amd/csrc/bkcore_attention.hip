@@ -13,6 +13,9 @@ inline bool rows_aligned(const Heads &x, int dtype) {
   return aligned16(x.p) && x.b % v == 0 && x.h % v == 0 && x.t % v == 0;
 }
 
+// a tile of 128 rows within 32-bit offsets
+inline bool near(const Heads &x) { return x.t >= 0 && x.t < (1 << 24); }
+
 int check(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D, int64_t window, int64_t sinks, float scale) {
   if (!elem_size(dtype) || B < 0 || H < 1 || Hk < 1 || H % Hk || L < 0 || D < 1 || D > BKCORE_ATTENTION_MAX_HEAD_DIM)
     return BKCORE_EINVAL;
@@ -79,6 +82,7 @@ extern "C" int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t 
   a.o = out; a.lo = out_lo; a.lse = lse; a.lengths = lengths;
   a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.L = (int)L; a.D = (int)D; a.S = (int)(sinks < L ? sinks : L);
   a.W = (int)(window < L ? window : L); a.scale = scale;
+  if (!near(a.k) || !near(a.v)) return BKCORE_EINVAL;
   const bool vec = D % 8 == 0 && rows_aligned(a.q, dtype) && rows_aligned(a.k, dtype) && rows_aligned(a.v, dtype) &&
                    aligned16(out) && aligned16(out_lo);
   BK_WITH_TYPE(dtype, attn_forward<T>(a, padded(D), vec, (hipStream_t)stream));
@@ -118,6 +122,7 @@ extern "C" int bkcore_sliding_attention_backward(
   a.nsplit = sink_splits(B, Hk, L, a.W, a.S);
   a.delta = (float *)workspace;
   a.part = a.delta + (((size_t)B * H * L + 3) & ~(size_t)3);
+  if (!near(a.q) || !near(a.k) || !near(a.v) || !near(a.dout)) return BKCORE_EINVAL;
   const bool vec = D % 8 == 0 && rows_aligned(a.q, dtype) && rows_aligned(a.k, dtype) && rows_aligned(a.v, dtype) &&
                    rows_aligned(a.dout, dtype) && aligned16(out) && aligned16(out_lo) && aligned16(dq) && aligned16(dk) && aligned16(dv);
   BK_WITH_TYPE(dtype, attn_backward<T>(a, padded(D), vec, (hipStream_t)stream));

@@ -50,11 +50,25 @@ __device__ __forceinline__ Frag<T> load8(const T *row, int c, int D) {
   }
   return f;
 }
-template <typename T>
+// (VEC: D is a multiple of 8, so the piece is inside or outside as a whole and is selected in 32-bit words.)
+template <typename T, bool VEC>
 __device__ __forceinline__ Frag<T> zero_unless(const Frag<T> &f, bool row_ok, int c, int D) {
   Frag<T> r;
+  if constexpr (VEC) {
+    constexpr int N = 8 * (int)sizeof(T) / 4;
+    union {
+      typename Frag<T>::vec v;
+      unsigned w[N];
+    } a, b;
+    a.v = f.v;
+    const bool in = row_ok & (c < D);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = row_ok && c + i < D ? f.v[i] : (T)0.0f;
+    for (int i = 0; i < N; ++i) b.w[i] = in ? a.w[i] : 0u;
+    r.v = b.v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = row_ok && c + i < D ? f.v[i] : (T)0.0f;
+  }
   return r;
 }
 
@@ -64,13 +78,15 @@ struct Tile {
   static constexpr int CH = DP / 8, N = (ROWS * CH + THREADS - 1) / THREADS;
   static constexpr bool WHOLE = ROWS * CH % THREADS == 0;  // else the last pass is for some of the threads
   Frag<T> r[N];
+  // A uniform 64-bit base and a 32-bit offset (the host keeps ROWS strides below 2^31); rows behind the last one repeat it.
   __device__ __forceinline__ void load(const T *base, long stride, long row0, long rows, int D, int tid) {
+    const T *tile = base + row0 * stride;
+    const unsigned most = (unsigned)(rows - 1 - row0 < ROWS ? rows - 1 - row0 : ROWS);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int i = tid + k * THREADS;
-      long row = row0 + i / CH;
-      row = row < rows ? row : rows - 1;
-      r[k] = load8<T, VEC>(base + row * stride, (i % CH) * 8, D);
+      const unsigned row = min((unsigned)(i / CH), most);
+      r[k] = load8<T, VEC>(tile + row * (unsigned)stride, (i % CH) * 8, D);
     }
   }
   __device__ __forceinline__ void store(T *lds, long row0, long rows, int D, int tid) const {
@@ -78,7 +94,7 @@ struct Tile {
     for (int k = 0; k < N; ++k) {
       const int i = tid + k * THREADS, row = i / CH, c = (i % CH) * 8;
       if (!WHOLE && i >= ROWS * CH) break;
-      const Frag<T> f = zero_unless(r[k], row0 + row < rows, c, D);
+      const Frag<T> f = zero_unless<T, VEC>(r[k], row0 + row < rows, c, D);
       *reinterpret_cast<typename Frag<T>::vec *>(lds + row * (DP + pad<T>()) + c) = f.v;
     }
   }
@@ -202,7 +218,7 @@ __device__ __forceinline__ int tile_view(int q0, int q1, int j0, int j1, int W, 
   if (j0 > q1 || (q0 - j1 >= W && j0 >= S)) return 0;
   return j1 <= q0 && (q1 - j0 < W || j1 < S) ? 2 : 1;
 }
-__device__ __forceinline__ bool sees(int i, int j, int W, int S) { return j <= i && (i - j < W || j < S); }
+__device__ __forceinline__ bool sees(int i, int j, int W, int S) { return (j <= i) & ((i - j < W) | (j < S)); }
 
 // ---- forward: 4 waves x 32 queries; keys and values through LDS, the next tile on its way in registers.
 template <typename T, int DP, bool VEC>
@@ -234,7 +250,7 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
       for (int c = 0; c < NC; ++c)
         q[i][c] = load8<T, VEC>(qp + (long)min(row, len - 1) * a.q.t, c * 32 + g * 8, a.D);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) q[i][c] = zero_unless(q[i][c], row < len, c * 32 + g * 8, a.D);
+      for (int c = 0; c < NC; ++c) q[i][c] = zero_unless<T, VEC>(q[i][c], row < len, c * 32 + g * 8, a.D);
     }
   }
   f32x4 o[ND][2];
@@ -283,12 +299,18 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
 #pragma unroll
       for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = s[k][i][r] * sc;
-          if (view == 1) x = sees(qi, j0 + 16 * k + 4 * g + r, a.W, a.S) ? x : -INF;
-          s[k][i][r] = x;
-          top = fmaxf(top, x);
-        }
+        for (int r = 0; r < 4; ++r) s[k][i][r] *= sc;
+      if (view == 1) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[k][i][r] = sees(qi, j0 + 16 * k + 4 * g + r, a.W, a.S) ? s[k][i][r] : -INF;
+      }
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[k][i][r]);
       top = fmaxf(mx[i], col_max(top));
       const float ref = top == -INF ? 0.0f : top, alpha = exp2_fast(mx[i] - ref);
       mx[i] = top;
@@ -415,8 +437,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        q[i][c] = zero_unless(q[i][c], row < len, c * 32 + g * 8, a.D);
-        go[i][c] = zero_unless(go[i][c], row < len, c * 32 + g * 8, a.D);
+        q[i][c] = zero_unless<T, VEC>(q[i][c], row < len, c * 32 + g * 8, a.D);
+        go[i][c] = zero_unless<T, VEC>(go[i][c], row < len, c * 32 + g * 8, a.D);
       }
     }
 #pragma unroll
@@ -460,11 +482,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
         for (int i = 0; i < 2; ++i) {
           const int qi = w0 + 16 * i + m;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = exp2_fast(fmaf(s[i][r], sc, -lse[i])) * (dp[i][r] - delta[i]);
-            if (view == 1) x = sees(qi, j0 + 16 * (k + kk) + 4 * g + r, a.W, a.S) ? x : 0.0f;
-            ds[i].v[4 * kk + r] = (T)x;
+          for (int r = 0; r < 4; ++r) s[i][r] = fmaf(s[i][r], sc, -lse[i]);
+          if (view == 1) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[i][r] = sees(qi, j0 + 16 * (k + kk) + 4 * g + r, a.W, a.S) ? s[i][r] : -INF;
           }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ds[i].v[4 * kk + r] = (T)(exp2_fast(s[i][r]) * (dp[i][r] - delta[i]));
         }
       }
 #pragma unroll
@@ -499,7 +524,10 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
 template <typename T, int DP, bool VEC, bool SINK>
 __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
   constexpr int BQ = ATTN_BQ, ROWS = SINK ? SINK_TILE : BQ, LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32;
-  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD];
+  // At 128 elements of 16 bits the keys' fragments stay in registers and the values' in LDS: both in registers leave no
+  // room for two waves a SIMD.
+  constexpr bool VLDS = DP == 128 && sizeof(T) == 2 && !SINK;
+  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD], sV[VLDS ? ATTN_BK * LD : 8];
   __shared__ __attribute__((aligned(16))) float sL[ROWS], sD[ROWS];
   const int nk = SINK ? (a.S + 31) / 32 : (a.L + ATTN_BK - 1) / ATTN_BK, ns = SINK ? a.nsplit : 1;
   long w = work_item((long)a.B * a.Hk * nk * ns);
@@ -527,7 +555,14 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
   }
   const T *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
   const float sc = a.scale * LOG2E;
-  Frag<T> kf[2][NC], vf[2][NC];
+  Frag<T> kf[2][NC], vf[VLDS ? 1 : 2][VLDS ? 1 : NC];
+  if constexpr (VLDS) {  // the loop's first barrier lies in front of its first use
+    if (len > 0) {
+      Tile<T, ATTN_BK, DP, 256, VEC> t;
+      t.load(vp, a.v.t, tile * ATTN_BK, len, a.D, tid);
+      t.store(sV, tile * ATTN_BK, len, a.D, tid);
+    }
+  }
   f32x4 dk[ND][2], dv[ND][2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -539,12 +574,12 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         kf[i][c] = load8<T, VEC>(kp + r * a.k.t, c * 32 + g * 8, a.D);
-        vf[i][c] = load8<T, VEC>(vp + r * a.v.t, c * 32 + g * 8, a.D);
+        if constexpr (!VLDS) vf[i][c] = load8<T, VEC>(vp + r * a.v.t, c * 32 + g * 8, a.D);
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        kf[i][c] = zero_unless(kf[i][c], row < len, c * 32 + g * 8, a.D);
-        vf[i][c] = zero_unless(vf[i][c], row < len, c * 32 + g * 8, a.D);
+        kf[i][c] = zero_unless<T, VEC>(kf[i][c], row < len, c * 32 + g * 8, a.D);
+        if constexpr (!VLDS) vf[i][c] = zero_unless<T, VEC>(vf[i][c], row < len, c * 32 + g * 8, a.D);
       }
     }
   }
@@ -588,7 +623,10 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           mma(qf, kf[y][c], s[y]);
-          mma(gf, vf[y][c], dp[y]);
+          if constexpr (VLDS)
+            mma(gf, along<T, DP>(sV, wave * 32 + 16 * y, 32 * c, lane), dp[y]);
+          else
+            mma(gf, vf[y][c], dp[y]);
         }
       }
       const f32x4 ls = *reinterpret_cast<const f32x4 *>(&sL[sub + 16 * x + 4 * g]);
@@ -596,12 +634,23 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
+        for (int r = 0; r < 4; ++r) s[y][r] = fmaf(s[y][r], sc, -ls[r]);
+      if (view == 1) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[y][r] = sees(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? s[y][r] : -INF;
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float p = exp2_fast(fmaf(s[y][r], sc, -ls[r]));
-          if (view == 1) p = sees(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? p : 0.0f;
+          const float p = exp2_fast(s[y][r]);
           pf[y].v[4 * x + r] = (T)p;
           df[y].v[4 * x + r] = (T)(p * (dp[y][r] - de[r]));
         }
+      if constexpr (VLDS) __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
@@ -610,6 +659,9 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
       for (int y = 0; y < 2; ++y) {
         mma(gt, pf[y], dv[d][y]);
         mma(qt, df[y], dk[d][y]);
+      }
+      if constexpr (VLDS) {
+        if (d & 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -700,7 +752,7 @@ __global__ __launch_bounds__(256) void bk_attn_step_kernel(StepArgs a) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) q[c] = load8<T, VEC>(qp, c * 32 + g * 8, a.D);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) q[c] = zero_unless(q[c], m < nh, c * 32 + g * 8, a.D);
+    for (int c = 0; c < NC; ++c) q[c] = zero_unless<T, VEC>(q[c], m < nh, c * 32 + g * 8, a.D);
   }
   f32x4 o[ND];
 #pragma unroll
@@ -734,7 +786,7 @@ __global__ __launch_bounds__(256) void bk_attn_step_kernel(StepArgs a) {
       s[k] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        if (!VEC || a.D < DP) kr[k][c] = zero_unless(kr[k][c], true, c * 32 + g * 8, a.D);
+        if (!VEC || a.D < DP) kr[k][c] = zero_unless<T, VEC>(kr[k][c], true, c * 32 + g * 8, a.D);
         mma(kr[k][c], q[c], s[k]);
       }
     }
@@ -742,7 +794,7 @@ __global__ __launch_bounds__(256) void bk_attn_step_kernel(StepArgs a) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = lane + 64 * k, r = i / (DP / 8), c = (i % (DP / 8)) * 8;
-      const Frag<T> f = zero_unless(vr[k], t0 + r < to, c, a.D);
+      const Frag<T> f = zero_unless<T, VEC>(vr[k], t0 + r < to, c, a.D);
       *reinterpret_cast<typename Frag<T>::vec *>(sV + r * LD + c) = f.v;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
