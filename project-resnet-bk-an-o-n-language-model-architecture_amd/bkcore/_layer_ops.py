@@ -54,17 +54,6 @@ def no_grad_through(what: str, *tensors) -> None:
         raise RuntimeError(f"bkcore: {what} serves single tokens and has no gradient; call it under torch.no_grad()")
 
 
-FAR = 1 << 24     # strides between positions from here on are beyond the kernels' 32-bit offsets inside a tile
-
-
-def inner(t: torch.Tensor | None) -> torch.Tensor | None:
-    """The tensor itself when its last dimension has unit stride (and its positions lie near enough), else a contiguous
-    copy."""
-    if t is None or ((t.shape[-1] <= 1 or t.stride(-1) == 1) and (t.dim() < 2 or t.stride(-2) < FAR)):
-        return t
-    return t.contiguous()
-
-
 def wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -80,21 +69,6 @@ def lengths_arg(what: str, lengths: torch.Tensor | None, x: torch.Tensor, batch:
     if lengths.dtype != torch.int64:
         raise TypeError(f"bkcore: {what}: lengths are int32 or int64, not {lengths.dtype}")
     return lengths.clamp(0, longest).to(torch.int32)
-
-
-def once_only(what: str) -> None:
-    """First line of a backward pass: gradient mode is on there only under create_graph."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"bkcore: {what} has first derivatives only (create_graph is not supported)")
-
-
-def ptr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
-
-
-def strides(t: torch.Tensor | None) -> tuple:
-    """The two outer strides of a three-dimensional operand."""
-    return (0, 0) if t is None else t.stride()[:2]
 
 
 stream = torch._C._cuda_getCurrentRawStream     # of a device index: the handle alone, without a Stream object around it

@@ -43,7 +43,7 @@ EXPORTS = ("bkcore_forward", "bkcore_forward_clamped", "bkcore_forward_noalloc",
            "bkcore_error_string", "bkcore_abi_version")
 
 _lib = None
-_held = None
+_native = None
 
 
 def load():
@@ -62,17 +62,21 @@ def load():
     return L
 
 
-def load_held():
-    """The library with the interpreter lock kept during a call, for the layer operators: their calls check arguments,
-    launch and return, and in a backward pass, which runs on the autograd engine's thread, giving the lock away and
-    fetching it back costs more than the call (a layer norm step 148 -> 96 us on the host)."""
-    global _held
-    if _held is None:
+def load_native():
+    """The module of the layer operators' tensor functions (csrc/bkcore_torch.cpp)."""
+    global _native
+    if _native is None:
         load()
-        L = ctypes.PyDLL(LIB_PATH)
-        _declare(L)
-        _held = L
-    return _held
+        try:
+            from . import _bkcore_torch
+        except ImportError as e:
+            raise RuntimeError(
+                f"bkcore: _bkcore_torch.so is missing or does not load ({e}). Build it with `make -C <package>/csrc`; there "
+                "is no other path for the layer operators.") from e
+        if _bkcore_torch.abi_version() != ABI_VERSION:
+            raise RuntimeError(f"bkcore: ABI version mismatch (tensor functions {_bkcore_torch.abi_version()}, wrapper {ABI_VERSION})")
+        _native = _bkcore_torch
+    return _native
 
 
 def _declare(L):

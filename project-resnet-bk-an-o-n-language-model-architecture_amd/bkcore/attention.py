@@ -44,55 +44,6 @@ def _scale(what: str, scale, D: int) -> float:
     return scale
 
 
-class _SlidingAttentionFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks, scale, lengths, keep):
-        q, k, v = ops.inner(q), ops.inner(k), ops.inner(v)
-        B, H, T, D = q.shape
-        Hk = k.shape[1]
-        dev = q.device
-        o = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
-        lse = torch.empty(B * H * T, dtype=torch.float32, device=dev) if keep else None
-        lo = torch.empty_like(o) if keep and q.dtype != torch.float32 else None   # what rounding takes from the output
-        with ops.on_device(dev):
-            rc = _lib.load_held().bkcore_sliding_attention(
-                q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-                ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window, sinks, scale, o.data_ptr(), ops.ptr(lo), ops.ptr(lse),
-                ops.stream(dev.index))
-        if rc:
-            _lib.check(rc, "bkcore_sliding_attention")
-        if keep:
-            ctx.save_for_backward(q, k, v, o, lo, lse, lengths)
-            ctx.bk_args = window, sinks, scale
-        return o.transpose(1, 2)
-
-    @staticmethod
-    def backward(ctx, do):
-        ops.once_only("sliding_attention")
-        q, k, v, o, lo, lse, lengths = ctx.saved_tensors
-        window, sinks, scale = ctx.bk_args
-        do = ops.inner(do)
-        B, H, T, D = q.shape
-        Hk = k.shape[1]
-        dev = q.device
-        dq = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
-        dk = torch.empty(B, T, Hk, D, dtype=q.dtype, device=dev)
-        dv = torch.empty_like(dk)
-        L = _lib.load_held()
-        nbytes = L.bkcore_sliding_attention_backward_workspace_bytes(B, H, Hk, T, D, window, sinks)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with ops.on_device(dev):
-            rc = L.bkcore_sliding_attention_backward(
-                do.data_ptr(), *do.stride()[:3], q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(),
-                *v.stride()[:3], o.data_ptr(), ops.ptr(lo), lse.data_ptr(), ops.DTYPES[q.dtype], ops.ptr(lengths), B, H, Hk, T, D, window,
-                sinks, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes, ops.stream(dev.index))
-        if rc:
-            _lib.check(rc, "bkcore_sliding_attention_backward")
-        need = ctx.needs_input_grad
-        return (dq.transpose(1, 2) if need[0] else None, dk.transpose(1, 2) if need[1] else None,
-                dv.transpose(1, 2) if need[2] else None, None, None, None, None, None)
-
-
 def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
                       scale: float | None = None, lengths: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q (B, H, L, D) to k, v (B, Hk, L, D) of the same positions, H a multiple of Hk (neighbouring query heads
@@ -107,7 +58,9 @@ def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     window, sinks = _window(what, window, sinks)
     scale = _scale(what, scale, D)
     n = ops.lengths_arg(what, lengths, q, B, T)
-    return _SlidingAttentionFunction.apply(q, k, v, window, sinks, scale, n, ops.wants_grad(q, k, v))
+    with ops.on_device(q.device):
+        return _lib.load_native().sliding_attention(q, k, v, n, window, sinks, scale, ops.wants_grad(q, k, v),
+                                                    ops.stream(q.device.index))
 
 
 def _cache(what: str, q: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int) -> int:
@@ -132,20 +85,13 @@ def sliding_cache_fill(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
     and the last ``slots - sinks`` behind them.  Position p lives in slot p for p < sinks and in slot
     ``sinks + (p - sinks) % (slots - sinks)`` behind; slots of no position stay as they were."""
     what = "sliding_cache_fill"
-    code = _heads(what, k, k, v, 4)
+    _heads(what, k, k, v, 4)
     _, sinks = _window(what, 1, sinks)
     ops.no_grad_through(what, k, v)
-    cap = _cache(what, k, k, k_cache, v_cache, sinks)
-    B, Hk, T, D = k.shape
-    n = ops.lengths_arg(what, lengths, k, B, T)
-    k, v = ops.inner(k), ops.inner(v)
-    dev = k.device
-    with ops.on_device(dev):
-        rc = _lib.load_held().bkcore_sliding_cache_fill(
-            k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], k_cache.data_ptr(), *k_cache.stride()[:3],
-            v_cache.data_ptr(), *v_cache.stride()[:3], ops.ptr(n), code, B, Hk, T, cap, D, sinks, ops.stream(dev.index))
-    if rc:
-        _lib.check(rc, "bkcore_sliding_cache_fill")
+    _cache(what, k, k, k_cache, v_cache, sinks)
+    n = ops.lengths_arg(what, lengths, k, k.shape[0], k.shape[2])
+    with ops.on_device(k.device):
+        _lib.load_native().sliding_cache_fill(k, v, k_cache, v_cache, n, sinks, ops.stream(k.device.index))
 
 
 def sliding_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -155,32 +101,19 @@ def sliding_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
     (B,), which are written into the rolling caches (see ``sliding_cache_fill``; at least ``window + sinks`` slots) in place.
     A negative position leaves its sequence alone: output zero, cache as it was.  No gradient."""
     what = "sliding_attention_step"
-    code = _heads(what, q, k, v, 3)
+    _heads(what, q, k, v, 3)
     window, sinks = _window(what, window, sinks)
     ops.no_grad_through(what, q, k, v)
     cap = _cache(what, q, k, k_cache, v_cache, sinks)
     if cap < window + sinks:
         raise ValueError(f"bkcore: {what}: a window of {window} and {sinks} sinks need {window + sinks} slots, got {cap}")
-    B, H, D = q.shape
-    Hk = k.shape[1]
-    scale = _scale(what, scale, D)
-    ops.need_shape(what, "positions", positions, (B,))
+    scale = _scale(what, scale, q.shape[-1])
+    ops.need_shape(what, "positions", positions, (q.shape[0],))
     ops.need_device(q, positions)
     if positions.dtype == torch.int64:
         positions = positions.to(torch.int32)
     elif positions.dtype != torch.int32:
         raise TypeError(f"bkcore: {what}: positions are int32 or int64, not {positions.dtype}")
-    q, k, v, positions = ops.inner(q), ops.inner(k), ops.inner(v), positions.contiguous()
-    dev = q.device
-    o = torch.empty(B, H, D, dtype=q.dtype, device=dev)
-    L = _lib.load_held()
-    nbytes = L.bkcore_sliding_attention_step_workspace_bytes(B, H, Hk, cap, D, window, sinks)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with ops.on_device(dev):
-        rc = L.bkcore_sliding_attention_step(
-            q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], k_cache.data_ptr(),
-            *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], positions.data_ptr(), code, B, H, Hk, cap, D,
-            window, sinks, scale, o.data_ptr(), ops.ptr(ws), nbytes, ops.stream(dev.index))
-    if rc:
-        _lib.check(rc, "bkcore_sliding_attention_step")
-    return o
+    with ops.on_device(q.device):
+        return _lib.load_native().sliding_attention_step(q, k, v, k_cache, v_cache, positions, window, sinks, scale,
+                                                         ops.stream(q.device.index))
