@@ -22,6 +22,11 @@ forward signatures on top of the HIP operator.
                               gate, and the operator's backward receives a cotangent on ``G_ii`` only.  The two mixing
                               paths are stand-ins (causal softmax attention in windows; a causal running mean over the
                               sequence through the library's cumulative sum).
+                              ``local="sliding"`` and ``global_path="selective"`` put the library's own operators in
+                              their place (a sliding window with sinks; a ``SelectiveMixer``), with forms for single
+                              tokens; ``norm="kernel"`` its layer norm.
+  * ``SelectiveMixer``        a selective state space mixer: input projection, short causal convolution, selective scan
+                              gated by the projection's other half, output projection; ``step`` for single tokens.
   * ``LearnedTridiagonalGreen`` the Green-function step of the reference's hyperbolic BK-Core block
                               (src/models/phase8/bk_core_hyperbolic.py:282-286, 349-407): all three diagonals are
                               projections of the input (``he_diag_proj``, ``h0_super_proj``, ``h0_sub_proj``, same names and
@@ -35,8 +40,18 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .attention import sliding_attention, sliding_attention_step, sliding_cache_fill
 from .bk_core import BKCoreFunction, FusedBKLayerFunction, FusedSpectralOutputFunction
+from .norm import LayerNorm
 from .scan import fused_associative_scan
+from .selective import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+
+
+def make_norm(norm: str, d_model: int, eps: float = 1e-5) -> nn.Module:
+    """``"torch"``: nn.LayerNorm; ``"kernel"``: the same module on the library's kernel (GPU tensors only)."""
+    if norm not in ("torch", "kernel"):
+        raise ValueError(f"unknown norm {norm!r}")
+    return (LayerNorm if norm == "kernel" else nn.LayerNorm)(d_model, eps=eps)
 
 
 class BKCoreLayer(nn.Module):
@@ -125,11 +140,69 @@ class BKCoreLayer(nn.Module):
         return out if residual is None else residual + out
 
 
+class SelectiveMixer(nn.Module):
+    """A selective state space mixer over (B, L, d_model): ``in_proj`` to 2 d_inner channels, a causal convolution of
+    ``conv_width`` taps with silu over the first half, ``x_proj`` / ``dt_proj`` to the step, B_t and C_t, the scan gated by
+    silu of the second half, ``out_proj``.  A starts at -1 ... -d_state in every channel, the step between 1e-3 and 0.1."""
+
+    def __init__(self, d_model: int, d_inner: int | None = None, d_state: int = 16, conv_width: int = 4,
+                 dt_rank: int | None = None):
+        super().__init__()
+        self.d_inner = d_inner = 2 * d_model if d_inner is None else d_inner
+        self.d_state, self.conv_width = d_state, conv_width
+        self.dt_rank = dt_rank = max(1, (d_model + 15) // 16) if dt_rank is None else dt_rank
+        self.in_proj = nn.Linear(d_model, 2 * d_inner, bias=False)
+        self.conv_weight = nn.Parameter(torch.empty(d_inner, conv_width))
+        self.conv_bias = nn.Parameter(torch.zeros(d_inner))
+        self.x_proj = nn.Linear(d_inner, dt_rank + 2 * d_state, bias=False)
+        self.dt_proj = nn.Linear(dt_rank, d_inner)                         # its bias enters the scan with the step
+        self.A_log = nn.Parameter(torch.log(torch.arange(1.0, d_state + 1)).repeat(d_inner, 1))
+        self.D = nn.Parameter(torch.ones(d_inner))
+        self.out_proj = nn.Linear(d_inner, d_model, bias=False)
+        nn.init.uniform_(self.conv_weight, -conv_width ** -0.5, conv_width ** -0.5)
+        with torch.no_grad():
+            step = torch.exp(torch.empty(d_inner).uniform_(-6.9, -2.3))
+            self.dt_proj.bias.copy_(step + torch.log(-torch.expm1(-step)))  # softplus of it is the step
+
+    def _projections(self, u: torch.Tensor):
+        dt, B, C = self.x_proj(u).split([self.dt_rank, self.d_state, self.d_state], dim=-1)
+        return F.linear(dt, self.dt_proj.weight), B, C
+
+    def new_state(self, batch: int, device, dtype: torch.dtype = torch.float32):
+        """Zero state in front of the first token: the convolution's last inputs (in the activations' type) and the scan's
+        state (float32)."""
+        return (torch.zeros(batch, self.conv_width - 1, self.d_inner, dtype=dtype, device=device),
+                torch.zeros(batch, self.d_inner, self.d_state, dtype=torch.float32, device=device))
+
+    def forward(self, x: torch.Tensor, lengths: torch.Tensor | None = None, state=None, return_state: bool = False):
+        """x (B, L, d_model); ``lengths`` (B,) of a right-padded batch; ``state`` to go on from, ``return_state`` to get the
+        one behind the last position."""
+        v, z = self.in_proj(x).chunk(2, dim=-1)
+        conv_state, ssm_state = (None, None) if state is None else state
+        u = causal_conv(v, self.conv_weight, self.conv_bias, "silu", lengths, conv_state, return_state)
+        u, conv_out = u if return_state else (u, None)
+        delta, B, C = self._projections(u)
+        y = selective_scan(u, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias, True, lengths, ssm_state,
+                           return_state)
+        y, ssm_out = y if return_state else (y, None)
+        y = self.out_proj(y)
+        return (y, (conv_out, ssm_out)) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state) -> torch.Tensor:
+        """One token of each sequence, x (B, d_model); ``state`` is updated in place."""
+        v, z = self.in_proj(x).chunk(2, dim=-1)
+        u = causal_conv_step(v, state[0], self.conv_weight, self.conv_bias, "silu")
+        delta, B, C = self._projections(u)
+        return self.out_proj(selective_scan_step(u, state[1], delta, -torch.exp(self.A_log), B, C, self.D, z,
+                                                 self.dt_proj.bias, True))
+
+
 class HybridGatedMixing(nn.Module):
-    def __init__(self, d_model: int, soft_cap: float = 30.0):
+    def __init__(self, d_model: int, soft_cap: float = 30.0, norm: str = "torch"):
         super().__init__()
         self.gate_sensitivity = nn.Parameter(torch.tensor(1.0))            # hybrid_attention.py:52
-        self.layer_norm = nn.LayerNorm(d_model, eps=1e-5)                  # :55
+        self.layer_norm = make_norm(norm, d_model, eps=1e-5)               # :55
         self.soft_cap = soft_cap                                           # :58
 
     def _cap(self, t: torch.Tensor) -> torch.Tensor:                       # :84-86, :110-112
@@ -150,23 +223,44 @@ class HybridGatedMixing(nn.Module):
 
 class BKHybridLayer(BKCoreLayer):
     """x -> v_proj -> operator -> G_ii -> gate between a local and a global mixing path of x.  ``output_proj`` and
-    ``bk_scale`` exist (as in the reference layer, whose state_dict has them) and are unused on this path."""
+    ``bk_scale`` exist (as in the reference layer, whose state_dict has them) and are unused on this path.
+
+    ``local``: ``"windows"``, causal attention inside blocks of ``window``, or ``"sliding"``, where every position sees the
+    last ``window`` ones and the first ``sinks``.  ``global_path``: ``"mean"``, a causal running mean, or ``"selective"``, a
+    ``SelectiveMixer``.  The new ones run on GPU tensors only."""
 
     def __init__(self, d_model: int, n_seq: int, num_heads: int = 8, window: int = 32, rank: int = 16,
-                 v_max: float = 5.0, fused: bool = False):
+                 v_max: float = 5.0, fused: bool = False, local: str = "windows", sinks: int = 0,
+                 global_path: str = "mean", norm: str = "torch"):
         super().__init__(d_model, n_seq, v_max=v_max, feature_clamp=5.0, fused=fused)
         if d_model % num_heads:
             raise ValueError("d_model must be a multiple of num_heads")
-        self.num_heads, self.window = num_heads, window
-        self.hybrid_attn = HybridGatedMixing(d_model)
+        if local not in ("windows", "sliding"):
+            raise ValueError(f"unknown local path {local!r}")
+        if global_path not in ("mean", "selective"):
+            raise ValueError(f"unknown global path {global_path!r}")
+        if sinks and local != "sliding":
+            raise ValueError("sinks belong to the sliding local path")
+        self.num_heads, self.window, self.local, self.sinks = num_heads, window, local, sinks
+        self.hybrid_attn = HybridGatedMixing(d_model, norm=norm)
         # stand-ins for HyperbolicMultiHeadAttention (windowed, causal) and AdaptiveRankSemiseparableLayer
         self.local_qkv = nn.Linear(d_model, 3 * d_model, bias=False)
         self.local_out = nn.Linear(d_model, d_model, bias=False)
-        self.global_in = nn.Linear(d_model, rank, bias=False)
-        self.global_out = nn.Linear(rank, d_model)
+        self.selective = SelectiveMixer(d_model) if global_path == "selective" else None
+        if self.selective is None:
+            self.global_in = nn.Linear(d_model, rank, bias=False)
+            self.global_out = nn.Linear(rank, d_model)
+
+    def _heads(self, x: torch.Tensor):
+        """x (B, N, D) -> q, k, v (B, heads, N, D / heads), views of one projection."""
+        B, N, D = x.shape
+        return self.local_qkv(x).view(B, N, 3, self.num_heads, D // self.num_heads).permute(2, 0, 3, 1, 4)
 
     def local_path(self, x: torch.Tensor) -> torch.Tensor:
         B, N, D = x.shape
+        if self.local == "sliding":
+            o = sliding_attention(*self._heads(x), self.window, self.sinks)
+            return self.local_out(o.transpose(1, 2).reshape(B, N, D))
         W = self.window
         pad = (W - N % W) % W                                              # hybrid_attention.py:93-100
         xp = F.pad(x, (0, 0, 0, pad)) if pad else x
@@ -175,7 +269,32 @@ class BKHybridLayer(BKCoreLayer):
         o = F.scaled_dot_product_attention(q, k, v, is_causal=True)        # causal inside each window (:103)
         return self.local_out(o.transpose(1, 2).reshape(B, nw * W, D))[:, :N]
 
+    def new_local_cache(self, batch: int, device, dtype: torch.dtype = torch.float32):
+        """Empty rolling caches of the sliding local path's keys and values."""
+        if self.local != "sliding":
+            raise ValueError("only the sliding local path has a cache")
+        shape = (batch, self.num_heads, self.window + self.sinks, self.d_model // self.num_heads)
+        return torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
+
+    @torch.no_grad()
+    def local_prefill(self, x: torch.Tensor, cache, lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """The sliding local path over prompts (B, N, D) of ``lengths``, whose keys and values go into ``cache``."""
+        B, N, D = x.shape
+        q, k, v = self._heads(x)
+        sliding_cache_fill(k, v, *cache, lengths, self.sinks)
+        o = sliding_attention(q, k, v, self.window, self.sinks, lengths=lengths)
+        return self.local_out(o.transpose(1, 2).reshape(B, N, D))
+
+    @torch.no_grad()
+    def local_step(self, x: torch.Tensor, cache, positions: torch.Tensor) -> torch.Tensor:
+        """The sliding local path for one token of each sequence, x (B, D) at ``positions`` (B,); ``cache`` is updated."""
+        B, D = x.shape
+        q, k, v = self.local_qkv(x).view(B, 3, self.num_heads, D // self.num_heads).unbind(1)
+        return self.local_out(sliding_attention_step(q, k, v, *cache, positions, self.window, self.sinks).reshape(B, D))
+
     def global_path(self, x: torch.Tensor) -> torch.Tensor:
+        if self.selective is not None:
+            return self.selective(x)
         u = self.global_in(x)                                              # (B, N, rank)
         csum = fused_associative_scan(u, dim=1) if u.is_cuda else torch.cumsum(u, dim=1)   # ar_ssm_layer.py:517-525
         pos = torch.arange(1, x.shape[1] + 1, device=x.device, dtype=u.dtype)

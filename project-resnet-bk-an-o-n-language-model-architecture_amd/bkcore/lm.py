@@ -6,7 +6,8 @@ token + position embedding, pre-norm residual blocks whose mixing path is the BK
 network, final LayerNorm, vocabulary head).  ``hybrid=True`` selects what configs/phase7_small.yaml:11 selects in the
 reference (``use_hybrid_attention``): the block's mixing path is gated by the resolvent diagonal
 (``bkcore.layers.BKHybridLayer``: the reference's gate, resnet_bk.py:172-185 and hybrid_attention.py:117-143, around
-stand-in local and global paths), the features go unused and the operator's backward sees a cotangent on G_ii alone.
+stand-in local and global paths, or the library's sliding-window attention and
+selective mixer: ``local``, ``sinks``, ``global_path``), the features go unused and the operator's backward sees a cotangent on G_ii alone.
 MoE routing and the HTT embedding are not part of it.  What it exercises is the operator inside a real backward pass and, with more than one
 process, the data-parallel gradient all-reduce around it.
 """
@@ -16,7 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .layers import BKCoreLayer, BKHybridLayer
+from .layers import BKCoreLayer, BKHybridLayer, make_norm
 
 
 class ResNetBKBlock(nn.Module):
@@ -24,14 +25,18 @@ class ResNetBKBlock(nn.Module):
     (src/models/moe.py:61-69 with num_experts = 1: the softmax over one gate is 1, so the layer is its one expert)."""
 
     def __init__(self, d_model: int, n_seq: int, ffn_mult: int = 4, fused: bool = False, ffn_activation: str = "gelu",
-                 hybrid: bool = False):
+                 hybrid: bool = False, norm: str = "torch", local: str = "windows", sinks: int = 0,
+                 global_path: str = "mean"):
         super().__init__()
         if ffn_activation not in ("gelu", "relu"):
             raise ValueError(f"unknown ffn_activation {ffn_activation!r}")
-        self.layer_norm = nn.LayerNorm(d_model)
+        if not hybrid and (local, sinks, global_path) != ("windows", 0, "mean"):
+            raise ValueError("local, sinks and global_path belong to the hybrid layer")
+        self.layer_norm = make_norm(norm, d_model)
         self.hybrid = hybrid
         if hybrid:      # no feed-forward branch: the reference builds none for a hybrid layer (resnet_bk.py:61-82)
-            self.bk_layer = BKHybridLayer(d_model, n_seq, fused=fused)
+            self.bk_layer = BKHybridLayer(d_model, n_seq, fused=fused, local=local, sinks=sinks, global_path=global_path,
+                                          norm=norm)
             self.ffn = None
             return
         self.bk_layer = BKCoreLayer(d_model, n_seq, fused=fused)
@@ -49,15 +54,17 @@ class ResNetBKBlock(nn.Module):
 
 class SmallResNetBKLM(nn.Module):
     def __init__(self, vocab_size: int = 50257, d_model: int = 256, n_layers: int = 4, n_seq: int = 256,
-                 fused: bool = False, ffn_mult: int = 4, ffn_activation: str = "gelu", hybrid: bool = False):
+                 fused: bool = False, ffn_mult: int = 4, ffn_activation: str = "gelu", hybrid: bool = False,
+                 norm: str = "torch", local: str = "windows", sinks: int = 0, global_path: str = "mean"):
         super().__init__()
         self.n_seq = n_seq
         self.token_embedding = nn.Embedding(vocab_size, d_model)
         self.position_embedding = nn.Embedding(n_seq, d_model)
         self.blocks = nn.ModuleList([ResNetBKBlock(d_model, n_seq, ffn_mult=ffn_mult, fused=fused,
-                                                   ffn_activation=ffn_activation, hybrid=hybrid)
+                                                   ffn_activation=ffn_activation, hybrid=hybrid, norm=norm, local=local,
+                                                   sinks=sinks, global_path=global_path)
                                      for _ in range(n_layers)])
-        self.layer_norm_final = nn.LayerNorm(d_model)
+        self.layer_norm_final = make_norm(norm, d_model)
         self.lm_head = nn.Linear(d_model, vocab_size)
         nn.init.normal_(self.token_embedding.weight, std=0.02)
         nn.init.normal_(self.position_embedding.weight, std=0.02)

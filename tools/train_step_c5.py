@@ -25,6 +25,10 @@ def main(argv=None, operator=None):
     ap.add_argument("--graph", action="store_true",
                     help="capture the whole step (forward, backward, clip, AdamW) in one HIP graph and replay it (1 GPU)")
     ap.add_argument("--hybrid", action="store_true", help="G_ii gates the mixing path (use_hybrid_attention)")
+    ap.add_argument("--local", default="windows", choices=["windows", "sliding"], help="with --hybrid: the local path")
+    ap.add_argument("--sinks", type=int, default=0, help="with --local sliding: first tokens that stay visible")
+    ap.add_argument("--global-path", default="mean", choices=["mean", "selective"], help="with --hybrid: the global path")
+    ap.add_argument("--norm", default="torch", choices=["torch", "kernel"], help="layer norms: tensor library or library kernel")
     ap.add_argument("--device", default="cuda", choices=["cuda", "cpu"])
     ap.add_argument("--force-dist", action="store_true",
                     help="a single rank also initialises the process group and wraps the model in DDP (rehearses the "
@@ -53,7 +57,8 @@ def main(argv=None, operator=None):
     from bkcore.lm import SmallResNetBKLM, training_step
     torch.manual_seed(0)
     model = SmallResNetBKLM(vocab_size=args.vocab, d_model=args.d_model, n_layers=args.layers, n_seq=args.n_seq,
-                            fused=args.fused, hybrid=args.hybrid).to(device)
+                            fused=args.fused, hybrid=args.hybrid, norm=args.norm, local=args.local, sinks=args.sinks,
+                            global_path=args.global_path).to(device)
     if operator is not None:
         model.set_bk_core(operator)
     if dist_on:
@@ -102,7 +107,7 @@ def main(argv=None, operator=None):
     if rank == 0:
         line = ({"metric": "resnet_bk_small_lm_train_tokens_per_sec", "value": world * args.batch * n_seq * args.steps / dt,
                           "unit": "tokens/s", "n_gpus": world, "steps": args.steps, "ms_per_step": dt / args.steps * 1e3,
-                          "final_loss": float(loss), "fused_layer": bool(args.fused), "hybrid": bool(args.hybrid), "hip_graph": bool(args.graph),
+                          "final_loss": float(loss), "fused_layer": bool(args.fused), "hybrid": bool(args.hybrid), "local": args.local, "global_path": args.global_path, "norm": args.norm, "hip_graph": bool(args.graph),
                  "device": args.device, "ddp": bool(dist_on), "config": {"workload": f"phase7_small dims: d_model {args.d_model}, {args.layers} layers, n_seq {n_seq}, "
                           f"batch {args.batch}/GPU, vocab {args.vocab}, AdamW 1e-4, clip 1.0; dummy tokens", "parallelism": f"dp{world}"}})
         print(json.dumps(line), flush=True)
