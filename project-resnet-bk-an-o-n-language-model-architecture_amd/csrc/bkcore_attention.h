@@ -21,7 +21,9 @@ struct AttnArgs {
   const int *lengths;
   int B, H, Hk, L, D, W, S;
   float scale;
-  int nsplit;  // sinks' gradient: stretches of queries behind the first key tile's own
+  int nsplit;         // sinks' gradient: stretches of queries behind the first key tile's own ...
+  long rest;          // ... which end here
+  int wide_q, wide_k; // 128 queries / keys a workgroup, else 64
 };
 
 struct StepArgs {
@@ -33,10 +35,7 @@ struct StepArgs {
   float scale;
 };
 
-// Queries of a forward / dq workgroup, keys of a dk, dv workgroup and queries of one of its tiles.
-constexpr int ATTN_BM = 128, ATTN_BK = 128, ATTN_BQ = 32;
-// First query that only the sinks of the first key tile are left for (window W): behind the tile's own queries.
-inline long __host__ __device__ sink_rest(long W) { return ((ATTN_BK - 1 + W - 1) / ATTN_BQ + 1) * ATTN_BQ; }
+constexpr int ATTN_BQ = 32;  // queries of one tile of a dk, dv workgroup
 constexpr int SINK_TILE = 4 * ATTN_BQ;  // queries a workgroup of the sinks' gradient takes at once: 32 a wave
 
 template <typename T>

@@ -24,11 +24,18 @@ int check(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D, int
   return BKCORE_OK;
 }
 
+// 128 queries (keys) a workgroup read a key (query) tile half as often as 64; fewer workgroups than fill the GPU twice are
+// better off as twice as many of the short ones.
+inline int wide(int64_t heads, int64_t L) { return heads * ((L + 127) / 128) >= 256; }
+
+// First query that only the sinks of the first key tile are left for: behind the tile's own queries.
+inline int64_t sink_rest(int64_t W, int wide_k) { return ((64 * (1 + wide_k) - 1 + W - 1) / ATTN_BQ + 1) * ATTN_BQ; }
+
 // Stretches of queries for the sinks' gradient: about two workgroups a CU together, at least 512 queries each.
 inline int sink_splits(int64_t B, int64_t Hk, int64_t L, int64_t W, int64_t S) {
-  const int64_t rest = L - sink_rest(W);
+  const int64_t rest = L - sink_rest(W, wide(B * Hk, L));
   if (S == 0 || rest <= 0) return 0;
-  int64_t n = 512 / (B * Hk * ((S + 31) / 32));
+  int64_t n = 512 / (B * Hk * (S > 16 ? (S + 31) / 32 : 1));
   const int64_t most = (rest + 511) / 512;
   if (n > most) n = most;
   return n < 1 ? 1 : (int)n;
@@ -74,7 +81,7 @@ extern "C" int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t 
   if (rc) return rc;
   if (B == 0 || L == 0) return BKCORE_OK;
   if (!q || !k || !v || !out) return BKCORE_EINVAL;
-  if (B * H * ((L + ATTN_BM - 1) / ATTN_BM) > 2147483000LL) return BKCORE_EINVAL;
+  if (B * H * ((L + 63) / 64) > 2147483000LL) return BKCORE_EINVAL;
   AttnArgs a{};
   a.q = {q, q_batch, q_head, q_time};
   a.k = {k, k_batch, k_head, k_time};
@@ -82,6 +89,7 @@ extern "C" int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t 
   a.o = out; a.lo = out_lo; a.lse = lse; a.lengths = lengths;
   a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.L = (int)L; a.D = (int)D; a.S = (int)(sinks < L ? sinks : L);
   a.W = (int)(window < L ? window : L); a.scale = scale;
+  a.wide_q = wide(B * H, L);
   if (!near(a.k) || !near(a.v)) return BKCORE_EINVAL;
   const bool vec = D % 8 == 0 && rows_aligned(a.q, dtype) && rows_aligned(a.k, dtype) && rows_aligned(a.v, dtype) &&
                    aligned16(out) && aligned16(out_lo);
@@ -108,7 +116,7 @@ extern "C" int bkcore_sliding_attention_backward(
   if (rc) return rc;
   if (B == 0 || L == 0) return BKCORE_OK;
   if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return BKCORE_EINVAL;
-  if (B * H * L > 2147483000LL * 16) return BKCORE_EINVAL;
+  if (B * H * L > 2147483000LL * 16 || B * H * ((L + 63) / 64) > 2147483000LL) return BKCORE_EINVAL;
   if (!workspace || workspace_bytes < bkcore_sliding_attention_backward_workspace_bytes(B, H, Hk, L, D, window, sinks))
     return BKCORE_EWORKSPACE;
   AttnArgs a{};
@@ -119,6 +127,9 @@ extern "C" int bkcore_sliding_attention_backward(
   a.out = out; a.lo = const_cast<void *>(out_lo); a.lse = const_cast<float *>(lse); a.lengths = lengths; a.dq = dq; a.dk = dk; a.dv = dv;
   a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.L = (int)L; a.D = (int)D; a.S = (int)(sinks < L ? sinks : L);
   a.W = (int)(window < L ? window : L); a.scale = scale;
+  a.wide_q = wide(B * H, L);
+  a.wide_k = wide(B * Hk, L);
+  a.rest = sink_rest(a.W, a.wide_k);
   a.nsplit = sink_splits(B, Hk, L, a.W, a.S);
   a.delta = (float *)workspace;
   a.part = a.delta + (((size_t)B * H * L + 3) & ~(size_t)3);

@@ -230,12 +230,12 @@ __device__ __forceinline__ int tile_view(int q0, int q1, int j0, int j1, int W, 
 }
 __device__ __forceinline__ bool sees(int i, int j, int W, int S) { return (j <= i) & ((i - j < W) | (j < S)); }
 
-// ---- forward: 4 waves x 32 queries; keys and values through LDS, the next tile on its way in registers.
-template <typename T, int DP, bool VEC>
+// ---- forward: 4 waves x 16 QB queries; keys and values through LDS, the next tile on its way in registers.
+template <typename T, int DP, bool VEC, int QB>
 __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
-  constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32;
+  constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32, WQ = 16 * QB, BM = 4 * WQ;
   __shared__ __attribute__((aligned(16))) T sK[BN * LD], sV[BN * LD];
-  const int nq = (a.L + ATTN_BM - 1) / ATTN_BM;
+  const int nq = (a.L + BM - 1) / BM;
   long w = work_item((long)a.B * a.H * nq);
   if (w < 0) return;
   const int G = a.H / a.Hk;
@@ -246,15 +246,15 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
   const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), h = hk * G + g_;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int len = row_length(a.lengths, b, a.L);
-  const int q0 = qt * ATTN_BM, q1 = min(q0 + ATTN_BM, len) - 1;
-  const int w0 = q0 + wave * 32, w1 = min(w0 + 32, len) - 1;  // the wave's own queries
+  const int q0 = qt * BM, q1 = min(q0 + BM, len) - 1;
+  const int w0 = q0 + wave * WQ, w1 = min(w0 + WQ, len) - 1;  // the wave's own queries
   const T *qp = head<T>(a.q, b, h), *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
   const float sc = a.scale * LOG2E;
 
-  Frag<T> q[2][NC];
+  Frag<T> q[QB][NC];
   if (q1 >= q0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < QB; ++i) {
       const int row = w0 + 16 * i + m;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -263,10 +263,10 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
       for (int c = 0; c < NC; ++c) q[i][c] = zero_unless<T, VEC>(q[i][c], row < len, c * 32 + g * 8, a.D);
     }
   }
-  f32x4 o[ND][2];
-  float mx[2], sum[2];
+  f32x4 o[ND][QB];
+  float mx[QB], sum[QB];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < QB; ++i) {
     mx[i] = -INF;
     sum[i] = 0.0f;
 #pragma unroll
@@ -291,19 +291,20 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
     }
     const int view = w1 >= w0 ? tile_view(w0, w1, j0, j0 + BN - 1, a.W, a.S) : 0;
     if (!view) continue;
-    f32x4 s[NK][2];
+    f32x4 s[NK][QB];
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
-      s[k][0] = s[k][1] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < QB; ++i) s[k][i] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const Frag<T> kf = along<T, DP>(sK, 16 * k, 32 * c, lane);
-        mma(kf, q[0][c], s[k][0]);
-        mma(kf, q[1][c], s[k][1]);
+#pragma unroll
+        for (int i = 0; i < QB; ++i) mma(kf, q[i][c], s[k][i]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < QB; ++i) {
       const int qi = w0 + 16 * i + m;
       float top = -INF;
 #pragma unroll
@@ -340,17 +341,19 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < NK; k += 2) {
-      const Frag<T> p0 = to_frag<T>(s[k][0], s[k + 1][0]), p1 = to_frag<T>(s[k][1], s[k + 1][1]);
+      Frag<T> p[QB];
+#pragma unroll
+      for (int i = 0; i < QB; ++i) p[i] = to_frag<T>(s[k][i], s[k + 1][i]);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const Frag<T> vf = across<T, DP>(sV, 16 * k, 16 * d, lane);
-        mma(vf, p0, o[d][0]);
-        mma(vf, p1, o[d][1]);
+#pragma unroll
+        for (int i = 0; i < QB; ++i) mma(vf, p[i], o[d][i]);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int row = w0 + 16 * i + m;
     const float l = col_sum(sum[i]);
     if (row < a.L) {
@@ -406,11 +409,11 @@ __global__ __launch_bounds__(256) void bk_attn_delta_kernel(AttnArgs a) {
 }
 
 // ---- dq: the forward's loop with two score products, dS^T in the lane, and K contracted over its rows.
-template <typename T, int DP, bool VEC>
+template <typename T, int DP, bool VEC, int QB>
 __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_kernel(AttnArgs a) {
-  constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32;
+  constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32, WQ = 16 * QB, BM = 4 * WQ;
   __shared__ __attribute__((aligned(16))) T sK[BN * LD], sV[BN * LD];
-  const int nq = (a.L + ATTN_BM - 1) / ATTN_BM;
+  const int nq = (a.L + BM - 1) / BM;
   long w = work_item((long)a.B * a.H * nq);
   if (w < 0) return;
   const int G = a.H / a.Hk;
@@ -421,15 +424,15 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
   const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), h = hk * G + g_;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int len = row_length(a.lengths, b, a.L);
-  const int q0 = qt * ATTN_BM, q1 = min(q0 + ATTN_BM, len) - 1;
-  const int w0 = q0 + wave * 32, w1 = min(w0 + 32, len) - 1;
+  const int q0 = qt * BM, q1 = min(q0 + BM, len) - 1;
+  const int w0 = q0 + wave * WQ, w1 = min(w0 + WQ, len) - 1;
   const T *qp = head<T>(a.q, b, h), *gp = head<T>(a.dout, b, h), *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
   const float sc = a.scale * LOG2E;
-  Frag<T> q[2][NC], go[2][NC];
-  float lse[2], delta[2];
-  f32x4 dq[ND][2];
+  Frag<T> q[QB][NC], go[QB][NC];
+  float lse[QB], delta[QB];
+  f32x4 dq[ND][QB];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int row = w0 + 16 * i + m;
     lse[i] = INF;
     delta[i] = 0.0f;
@@ -475,21 +478,23 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
     if (!view) continue;
 #pragma unroll
     for (int k = 0; k < NK; k += 2) {
-      Frag<T> ds[2], dl[2];
+      Frag<T> ds[QB], dl[QB];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        f32x4 s[2], dp[2];
-        s[0] = s[1] = dp[0] = dp[1] = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 s[QB], dp[QB];
+#pragma unroll
+        for (int i = 0; i < QB; ++i) s[i] = dp[i] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const Frag<T> kf = along<T, DP>(sK, 16 * (k + kk), 32 * c, lane), vf = along<T, DP>(sV, 16 * (k + kk), 32 * c, lane);
-          mma(kf, q[0][c], s[0]);
-          mma(kf, q[1][c], s[1]);
-          mma(vf, go[0][c], dp[0]);
-          mma(vf, go[1][c], dp[1]);
+#pragma unroll
+          for (int i = 0; i < QB; ++i) {
+            mma(kf, q[i][c], s[i]);
+            mma(vf, go[i][c], dp[i]);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < QB; ++i) {
           const int qi = w0 + 16 * i + m;
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[i][r] = fmaf(s[i][r], sc, -lse[i]);
@@ -507,7 +512,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
       for (int d = 0; d < ND; ++d) {
         const Frag<T> kf = across<T, DP>(sK, 16 * k, 16 * d, lane);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < QB; ++i) {
           mma(kf, ds[i], dq[d][i]);
           if constexpr (sizeof(T) == 2) mma(kf, dl[i], dq[d][i]);
         }
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int row = w0 + 16 * i + m;
     if (row < a.L) {
       T *op = (T *)a.dq + (((long)b * a.L + row) * a.H + h) * a.D;
@@ -530,20 +535,20 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
   }
 }
 
-// ---- dk, dv.  SINK false: 4 waves x 32 keys, all of them over the same 32 queries at a time, over the tile's own queries
+// ---- dk, dv.  SINK false: 4 waves x 16 KB keys, all of them over the same 32 queries at a time, over the tile's own queries
 // (its window) and the heads of the group.  SINK true: the sinks' part behind that -- the first 64 keys see all later
-// queries, so their loop is the whole sequence: it is cut into stretches, a wave takes 32 keys (keys 32 kh ...) and its own
+// queries, so their loop is the whole sequence: it is cut into stretches, a wave takes 16 KB of these keys and its own
 // 32 of every 128 queries, and leaves float32 sums that the join adds up in a fixed order.
 // part: (1 + 4 nsplit, B, Hk, S, 2, D); slot 0 is what the first key tile has from its own queries.
-template <typename T, int DP, bool VEC, bool SINK>
-__global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
-  constexpr int BQ = ATTN_BQ, ROWS = SINK ? SINK_TILE : BQ, LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32;
+template <typename T, int DP, bool VEC, bool SINK, int KB>
+__global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
+  constexpr int WK = 16 * KB, BK = 4 * WK, BQ = ATTN_BQ, ROWS = SINK ? SINK_TILE : BQ, LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32;
   // At 128 elements of 16 bits the keys' fragments stay in registers and the values' in LDS: both in registers leave no
   // room for two waves a SIMD.
-  constexpr bool VLDS = DP == 128 && sizeof(T) == 2 && !SINK;
-  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD], sV[VLDS ? ATTN_BK * LD : 8];
+  constexpr bool VLDS = KB == 2 && DP == 128 && sizeof(T) == 2 && !SINK;
+  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD], sV[VLDS ? BK * LD : 8];
   __shared__ __attribute__((aligned(16))) float sL[ROWS], sD[ROWS];
-  const int nk = SINK ? (a.S + 31) / 32 : (a.L + ATTN_BK - 1) / ATTN_BK, ns = SINK ? a.nsplit : 1;
+  const int nk = SINK ? (a.S + WK - 1) / WK : (a.L + BK - 1) / BK, ns = SINK ? a.nsplit : 1;
   long w = work_item((long)a.B * a.Hk * nk * ns);
   if (w < 0) return;
   const int tile = (int)(w % nk);
@@ -553,33 +558,33 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
   const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), G = a.H / a.Hk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int len = row_length(a.lengths, b, a.L);
-  const int key0 = SINK ? tile * 32 : tile * ATTN_BK + wave * 32;  // the wave's 32 keys
+  const int key0 = SINK ? tile * WK : tile * BK + wave * WK;  // the wave's first key
   const int sub = SINK ? wave * BQ : 0;                              // its queries inside the tile
   long q_from, q_to;
   if (SINK) {
-    const long rest = sink_rest(a.W), n = a.L > rest ? a.L - rest : 0;
+    const long rest = a.rest, n = a.L > rest ? a.L - rest : 0;
     const long per = ((n + ns - 1) / ns + ROWS - 1) / ROWS * ROWS;
     q_from = rest + split * per;
     q_to = q_from + per < len ? q_from + per : len;
   } else {
-    const int k0 = tile * ATTN_BK;
+    const int k0 = tile * BK;
     q_from = k0 / BQ * BQ;
-    q_to = ((long)k0 + ATTN_BK - 1 + a.W - 1) / BQ * BQ + BQ;
+    q_to = ((long)k0 + BK - 1 + a.W - 1) / BQ * BQ + BQ;
     q_to = q_to < len ? q_to : len;
   }
   const T *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
   const float sc = a.scale * LOG2E;
-  Frag<T> kf[2][NC], vf[VLDS ? 1 : 2][VLDS ? 1 : NC];
+  Frag<T> kf[KB][NC], vf[VLDS ? 1 : KB][VLDS ? 1 : NC];
   if constexpr (VLDS) {  // the loop's first barrier lies in front of its first use
     if (len > 0) {
-      Tile<T, ATTN_BK, DP, 256, VEC> t;
-      t.load(vp, a.v.t, tile * ATTN_BK, len, a.D, tid);
-      t.store(sV, tile * ATTN_BK, len, a.D, tid);
+      Tile<T, BK, DP, 256, VEC> t;
+      t.load(vp, a.v.t, tile * BK, len, a.D, tid);
+      t.store(sV, tile * BK, len, a.D, tid);
     }
   }
-  f32x4 dk[ND][2], dv[ND][2];
+  f32x4 dk[ND][KB], dv[ND][KB];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < KB; ++i) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d][i] = dv[d][i] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (len > 0) {
@@ -624,21 +629,22 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
     __syncthreads();
     if (it + 1 < total) fetch(it + 1);
     const int i0 = (int)qi + sub;
-    const int view = i0 < len && key0 < len ? tile_view(i0, i0 + BQ - 1, key0, key0 + 31, a.W, a.S) : 0;
+    const int view = i0 < len && key0 < len ? tile_view(i0, i0 + BQ - 1, key0, key0 + WK - 1, a.W, a.S) : 0;
     if (!view) continue;
-    Frag<T> pf[2], df[2], dl[2];
+    Frag<T> pf[KB], df[KB], dl[KB];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      f32x4 s[2], dp[2];  // of the key blocks: a lane holds four queries of one key
-      s[0] = s[1] = dp[0] = dp[1] = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 s[KB], dp[KB];  // of the key blocks: a lane holds four queries of one key
+#pragma unroll
+      for (int y = 0; y < KB; ++y) s[y] = dp[y] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const Frag<T> qf = along<T, DP>(sQ, sub + 16 * x, 32 * c, lane), gf = along<T, DP>(sG, sub + 16 * x, 32 * c, lane);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
+        for (int y = 0; y < KB; ++y) {
           mma(qf, kf[y][c], s[y]);
           if constexpr (VLDS)
-            mma(gf, along<T, DP>(sV, wave * 32 + 16 * y, 32 * c, lane), dp[y]);
+            mma(gf, along<T, DP>(sV, wave * WK + 16 * y, 32 * c, lane), dp[y]);
           else
             mma(gf, vf[y][c], dp[y]);
         }
@@ -646,18 +652,18 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
       const f32x4 ls = *reinterpret_cast<const f32x4 *>(&sL[sub + 16 * x + 4 * g]);
       const f32x4 de = *reinterpret_cast<const f32x4 *>(&sD[sub + 16 * x + 4 * g]);
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < KB; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[y][r] = fmaf(s[y][r], sc, -ls[r]);
       if (view == 1) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < KB; ++y)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             s[y][r] = sees(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? s[y][r] : -INF;
       }
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < KB; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float p = exp2_fast(s[y][r]);
@@ -670,7 +676,7 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
     for (int d = 0; d < ND; ++d) {
       const Frag<T> gt = across<T, DP>(sG, sub, 16 * d, lane), qt = across<T, DP>(sQ, sub, 16 * d, lane);
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
+      for (int y = 0; y < KB; ++y) {
         mma(gt, pf[y], dv[d][y]);
         mma(qt, df[y], dk[d][y]);
         if constexpr (sizeof(T) == 2) mma(qt, dl[y], dk[d][y]);
@@ -682,7 +688,7 @@ __global__ __launch_bounds__(256, DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2)
   }
   const bool parts = a.nsplit > 0;
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
+  for (int y = 0; y < KB; ++y) {
     const int key = key0 + 16 * y + m;
     if (SINK || (parts && key < a.S)) {
       if (key < a.S) {
@@ -910,28 +916,48 @@ __global__ __launch_bounds__(128) void bk_attn_step_join_kernel(StepArgs a) {
 
 template <typename T>
 void attn_forward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
-  const unsigned grid = work_grid((long)a.B * a.H * ((a.L + ATTN_BM - 1) / ATTN_BM));
-#define BK_LAUNCH(DP, VEC) hipLaunchKernelGGL((bk_attn_kernel<T, DP, VEC>), dim3(grid), dim3(256), 0, s, a)
+  const long heads = (long)a.B * a.H;
+#define BK_LAUNCH_Q(DP, VEC, QB)                                                                                     \
+  hipLaunchKernelGGL((bk_attn_kernel<T, DP, VEC, QB>), dim3(work_grid(heads * ((a.L + 64 * QB - 1) / (64 * QB)))),   \
+                     dim3(256), 0, s, a)
+#define BK_LAUNCH(DP, VEC)                   \
+  do {                                       \
+    if (a.wide_q) BK_LAUNCH_Q(DP, VEC, 2);   \
+    else BK_LAUNCH_Q(DP, VEC, 1);            \
+  } while (0)
   BK_ATTN_DP(BK_LAUNCH);
 #undef BK_LAUNCH
+#undef BK_LAUNCH_Q
 }
 
 template <typename T>
 void attn_backward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
-  const long rows = (long)a.B * a.H * a.L;
+  const long rows = (long)a.B * a.H * a.L, heads = (long)a.B * a.H, kheads = (long)a.B * a.Hk;
   const unsigned grid_d = (unsigned)((rows * (dp / 8) + 255) / 256);
-  const unsigned grid_q = work_grid((long)a.B * a.H * ((a.L + ATTN_BM - 1) / ATTN_BM));
-  const unsigned grid_k = work_grid((long)a.B * a.Hk * ((a.L + ATTN_BK - 1) / ATTN_BK));
-  const unsigned grid_s = work_grid((long)a.B * a.Hk * ((a.S + 31) / 32) * a.nsplit);
-#define BK_LAUNCH(DP, VEC)                                                                                      \
-  do {                                                                                                          \
-    hipLaunchKernelGGL((bk_attn_delta_kernel<T, DP, VEC>), dim3(grid_d), dim3(256), 0, s, a);                   \
-    hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, false>), dim3(grid_k), dim3(256), 0, s, a);              \
-    if (a.nsplit) hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, true>), dim3(grid_s), dim3(256), 0, s, a); \
-    hipLaunchKernelGGL((bk_attn_dq_kernel<T, DP, VEC>), dim3(grid_q), dim3(256), 0, s, a);                      \
+#define BK_LAUNCH_Q(DP, VEC, QB)                                                                                      \
+  hipLaunchKernelGGL((bk_attn_dq_kernel<T, DP, VEC, QB>), dim3(work_grid(heads * ((a.L + 64 * QB - 1) / (64 * QB)))), \
+                     dim3(256), 0, s, a)
+#define BK_LAUNCH_K(DP, VEC, KB)                                                                                      \
+  hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, false, KB>),                                                     \
+                     dim3(work_grid(kheads * ((a.L + 64 * KB - 1) / (64 * KB)))), dim3(256), 0, s, a)
+#define BK_LAUNCH_S(DP, VEC, KB)                                                                                      \
+  hipLaunchKernelGGL((bk_attn_dkv_kernel<T, DP, VEC, true, KB>),                                                      \
+                     dim3(work_grid(kheads * ((a.S + 16 * KB - 1) / (16 * KB)) * a.nsplit)), dim3(256), 0, s, a)
+#define BK_LAUNCH(DP, VEC)                                                                        \
+  do {                                                                                            \
+    hipLaunchKernelGGL((bk_attn_delta_kernel<T, DP, VEC>), dim3(grid_d), dim3(256), 0, s, a);     \
+    if (a.wide_k) BK_LAUNCH_K(DP, VEC, 2);                                                        \
+    else BK_LAUNCH_K(DP, VEC, 1);                                                                 \
+    if (a.nsplit && a.S > 16) BK_LAUNCH_S(DP, VEC, 2);                                            \
+    else if (a.nsplit) BK_LAUNCH_S(DP, VEC, 1);                                                   \
+    if (a.wide_q) BK_LAUNCH_Q(DP, VEC, 2);                                                        \
+    else BK_LAUNCH_Q(DP, VEC, 1);                                                                 \
   } while (0)
   BK_ATTN_DP(BK_LAUNCH);
 #undef BK_LAUNCH
+#undef BK_LAUNCH_Q
+#undef BK_LAUNCH_K
+#undef BK_LAUNCH_S
   if (a.nsplit) {
     const long per = (long)a.B * a.Hk * a.S * 2 * a.D;
     hipLaunchKernelGGL((bk_attn_sink_join_kernel<T>), dim3((unsigned)((per + 255) / 256)), dim3(256), 0, s, a);
