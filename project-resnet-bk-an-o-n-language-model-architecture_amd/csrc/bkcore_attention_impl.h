@@ -36,7 +36,7 @@ __device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &c
 }
 
 template <typename T>
-constexpr int pad() { return 16 / (int)sizeof(T); }  // elements that set LDS rows apart: 16 rows then cover all 64 banks
+constexpr int pad() { return sizeof(T) == 2 ? 16 : 4; }
 
 // Eight elements of row `row` (clamped by the caller to one that exists) from column c: raw, zeroed where not wanted.
 template <typename T, bool VEC>
@@ -509,12 +509,19 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
         }
       }
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const Frag<T> kf = across<T, DP>(sK, 16 * k, 16 * d, lane);
+      for (int d = 0; d < ND; d += 2) {  // two column blocks: four products between two on the same accumulator
+        const Frag<T> ka = across<T, DP>(sK, 16 * k, 16 * d, lane), kb = across<T, DP>(sK, 16 * k, 16 * d + 16, lane);
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
-          mma(kf, ds[i], dq[d][i]);
-          if constexpr (sizeof(T) == 2) mma(kf, dl[i], dq[d][i]);
+          mma(ka, ds[i], dq[d][i]);
+          mma(kb, ds[i], dq[d + 1][i]);
+        }
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int i = 0; i < QB; ++i) {
+            mma(ka, dl[i], dq[d][i]);
+            mma(kb, dl[i], dq[d + 1][i]);
+          }
         }
       }
     }
@@ -543,10 +550,12 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
 template <typename T, int DP, bool VEC, bool SINK, int KB>
 __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 256 ? 1 : 2) void bk_attn_dkv_kernel(AttnArgs a) {
   constexpr int WK = 16 * KB, BK = 4 * WK, BQ = ATTN_BQ, ROWS = SINK ? SINK_TILE : BQ, LD = DP + pad<T>(), ND = DP / 16, NC = DP / 32;
-  // At 128 elements of 16 bits the keys' fragments stay in registers and the values' in LDS: both in registers leave no
-  // room for two waves a SIMD.
+  // At 128 elements of 16 bits the values' fragments and half of the keys' wait in LDS, each lane's as it wants them: in
+  // registers they leave no room for two waves a SIMD, and a single spilled word costs more than these reads (its reload
+  // waits for the rows under way).
   constexpr bool VLDS = KB == 2 && DP == 128 && sizeof(T) == 2 && !SINK;
-  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD], sV[VLDS ? BK * LD : 8];
+  __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD];
+  __shared__ Frag<T> sF[VLDS ? 4 * 3 * NC * 64 : 1];
   __shared__ __attribute__((aligned(16))) float sL[ROWS], sD[ROWS];
   const int nk = SINK ? (a.S + WK - 1) / WK : (a.L + BK - 1) / BK, ns = SINK ? a.nsplit : 1;
   long w = work_item((long)a.B * a.Hk * nk * ns);
@@ -574,14 +583,8 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
   }
   const T *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
   const float sc = a.scale * LOG2E;
-  Frag<T> kf[KB][NC], vf[VLDS ? 1 : KB][VLDS ? 1 : NC];
-  if constexpr (VLDS) {  // the loop's first barrier lies in front of its first use
-    if (len > 0) {
-      Tile<T, BK, DP, 256, VEC> t;
-      t.load(vp, a.v.t, tile * BK, len, a.D, tid);
-      t.store(sV, tile * BK, len, a.D, tid);
-    }
-  }
+  Frag<T> kf[VLDS ? 1 : KB][NC], vf[VLDS ? 1 : KB][VLDS ? 1 : NC];
+  Frag<T> *mine = sF + (VLDS ? wave * 3 * NC * 64 + lane : 0);  // v of both key blocks, then k of the second
   f32x4 dk[ND][KB], dv[ND][KB];
 #pragma unroll
   for (int i = 0; i < KB; ++i) {
@@ -590,15 +593,24 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
     if (len > 0) {
       const int row = key0 + 16 * i + m;
       const long r = min(row, len - 1);
+      Frag<T> k_[NC], v_[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        kf[i][c] = load8<T, VEC>(kp + r * a.k.t, c * 32 + g * 8, a.D);
-        if constexpr (!VLDS) vf[i][c] = load8<T, VEC>(vp + r * a.v.t, c * 32 + g * 8, a.D);
+        k_[c] = load8<T, VEC>(kp + r * a.k.t, c * 32 + g * 8, a.D);
+        v_[c] = load8<T, VEC>(vp + r * a.v.t, c * 32 + g * 8, a.D);
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        kf[i][c] = zero_unless<T, VEC>(kf[i][c], row < len, c * 32 + g * 8, a.D);
-        if constexpr (!VLDS) vf[i][c] = zero_unless<T, VEC>(vf[i][c], row < len, c * 32 + g * 8, a.D);
+        k_[c] = zero_unless<T, VEC>(k_[c], row < len, c * 32 + g * 8, a.D);
+        v_[c] = zero_unless<T, VEC>(v_[c], row < len, c * 32 + g * 8, a.D);
+        if constexpr (VLDS) {
+          mine[(i * NC + c) * 64] = v_[c];
+          if (i == 0) kf[0][c] = k_[c];
+          else mine[(2 * NC + c) * 64] = k_[c];
+        } else {
+          kf[i][c] = k_[c];
+          vf[i][c] = v_[c];
+        }
       }
     }
   }
@@ -642,11 +654,13 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
         const Frag<T> qf = along<T, DP>(sQ, sub + 16 * x, 32 * c, lane), gf = along<T, DP>(sG, sub + 16 * x, 32 * c, lane);
 #pragma unroll
         for (int y = 0; y < KB; ++y) {
-          mma(qf, kf[y][c], s[y]);
-          if constexpr (VLDS)
-            mma(gf, along<T, DP>(sV, wave * WK + 16 * y, 32 * c, lane), dp[y]);
-          else
+          if constexpr (VLDS) {
+            mma(qf, y ? mine[(2 * NC + c) * 64] : kf[0][c], s[y]);
+            mma(gf, mine[(y * NC + c) * 64], dp[y]);
+          } else {
+            mma(qf, kf[y][c], s[y]);
             mma(gf, vf[y][c], dp[y]);
+          }
         }
       }
       const f32x4 ls = *reinterpret_cast<const f32x4 *>(&sL[sub + 16 * x + 4 * g]);
@@ -677,9 +691,12 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
       const Frag<T> gt = across<T, DP>(sG, sub, 16 * d, lane), qt = across<T, DP>(sQ, sub, 16 * d, lane);
 #pragma unroll
       for (int y = 0; y < KB; ++y) {
-        mma(gt, pf[y], dv[d][y]);
         mma(qt, df[y], dk[d][y]);
-        if constexpr (sizeof(T) == 2) mma(qt, dl[y], dk[d][y]);
+        mma(gt, pf[y], dv[d][y]);
+      }
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int y = 0; y < KB; ++y) mma(qt, dl[y], dk[d][y]);
       }
       if constexpr (VLDS) {
         if (d & 1) __builtin_amdgcn_sched_barrier(0);
