@@ -29,76 +29,124 @@ __device__ __forceinline__ float row_sum(float x, float *lds, int slot) {
   return s;
 }
 
-// Element i of thread t's E elements, V at a time: column ((i / V) * TPR + t) * V + i % V.
-template <typename T, int TPR, int E, int V>
+// A row over TPR threads: thread t's E elements, V = 16 bytes at a time, are columns ((i / V) * TPR + t) * V + i % V of the
+// whole pieces.  ALIGNED: rows start at 16-byte addresses and hold whole pieces only.  Otherwise pieces are read at any
+// address and the D % V columns behind them belong to the first threads, one each (element E).
+template <typename T, int TPR, int E, bool ALIGNED>
 struct Row {
-  RawVec<T, V> r[E / V];
-  __device__ __forceinline__ void load(const T *__restrict__ p, int t, int D) {
-#pragma unroll
-    for (int c = 0; c < E / V; ++c) {
-      const int col = (c * TPR + t) * V;
-      r[c].load(p + (col < D ? col : 0));
-    }
+  static constexpr int V = 16 / (int)sizeof(T), EX = ALIGNED ? E : E + 1;
+  LooseVec<T, V> r[E / V];
+  RawVec<T, V> ra[E / V];
+  T last;
+  static __device__ __forceinline__ int whole(int D) { return ALIGNED ? D : D / V * V; }
+  static __device__ __forceinline__ int column(int e, int t, int D) {
+    return e < E ? ((e / V) * TPR + t) * V + e % V : whole(D) + t;
   }
-  __device__ __forceinline__ void get(int t, int D, float (&v)[E]) const {
+  static __device__ __forceinline__ bool holds(int e, int t, int D) {
+    return e < E ? ((e / V) * TPR + t) * V < whole(D) : t < D - whole(D);
+  }
+  __device__ __forceinline__ void load(const T *__restrict__ p, int t, int D) {
+    const int Dv = whole(D);
+    if (ALIGNED || Dv > 0) {
+#pragma unroll
+      for (int c = 0; c < E / V; ++c) {
+        const int col = (c * TPR + t) * V;
+        if constexpr (ALIGNED) ra[c].load(p + (col < Dv ? col : 0));
+        else r[c].load(p + (col < Dv ? col : 0));
+      }
+    }
+    if constexpr (!ALIGNED) last = p[t < D - Dv ? Dv + t : 0];
+  }
+  __device__ __forceinline__ void get(int t, int D, float (&v)[EX]) const {
 #pragma unroll
     for (int c = 0; c < E / V; ++c) {
       float w[V];
-      r[c].get((c * TPR + t) * V < D, w);
+      if constexpr (ALIGNED) ra[c].get(holds(c * V, t, D), w);
+      else r[c].get(holds(c * V, t, D), w);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[c * V + i] = w[i];
+    }
+    if constexpr (!ALIGNED) v[E] = holds(E, t, D) ? (float)last : 0.0f;
+  }
+  // o[e] to the thread's columns of row p
+  static __device__ __forceinline__ void store(T *__restrict__ p, int t, int D, const float (&o)[EX]) {
+#pragma unroll
+    for (int c = 0; c < E / V; ++c) {
+      const int col = (c * TPR + t) * V;
+      if (col < whole(D)) {
+        float w[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = o[c * V + i];
+        if constexpr (ALIGNED) store_vec<T, V>(p + col, w);
+        else LooseVec<T, V>::store(p + col, w);
+      }
+    }
+    if constexpr (!ALIGNED) {
+      if (holds(E, t, D)) p[whole(D) + t] = (T)o[E];
+    }
+  }
+  // a parameter vector at the thread's columns
+  static __device__ __forceinline__ void param(const void *w, bool f32, int t, int D, float (&v)[EX]) {
+#pragma unroll
+    for (int c = 0; c < E / V; ++c) {
+      const int col = (c * TPR + t) * V;
+      float x[V];
+      if (col < whole(D)) {
+        load_param<T, V>(w, f32, col, x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[c * V + i] = x[i];
+    }
+    if constexpr (!ALIGNED) {
+      float x[1] = {0.0f};
+      if (holds(E, t, D)) load_param<T, 1>(w, f32, whole(D) + t, x);
+      v[E] = x[0];
     }
   }
 };
 
-template <typename T, int TPR, int E, int V>
+template <typename T, int TPR, int E, bool ALIGNED>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_kernel(
     const T *__restrict__ x, long ldx, const void *__restrict__ w, const void *__restrict__ b, int param_f32, float eps,
     long rows, int D, T *__restrict__ y, float *__restrict__ stats) {
+  typedef Row<T, TPR, E, ALIGNED> R;
   constexpr int RPB = TPR == 64 ? 4 : 1;  // rows per workgroup
   __shared__ float lds[2 * (TPR / 64)];
   const int t = TPR == 64 ? threadIdx.x & 63 : threadIdx.x;
   const long row = (long)blockIdx.x * RPB + (TPR == 64 ? threadIdx.x >> 6 : 0);
   if (row >= rows) return;  // uniform in the wave (TPR 64) or in the workgroup
-  float v[E];
-  Row<T, TPR, E, V> raw;
+  float v[R::EX], p[R::EX];
+  R raw;
   raw.load(x + row * ldx, t, D);
   raw.get(t, D, v);
   float s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < E; ++i) s += v[i];
+  for (int e = 0; e < R::EX; ++e) s += v[e];
   const float mean = row_sum<TPR>(s, lds, 0) / (float)D;
   float q = 0.0f;
 #pragma unroll
-  for (int c = 0; c < E / V; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float d = v[c * V + i] - mean;
-      if ((c * TPR + t) * V < D) q = fmaf(d, d, q);
-      v[c * V + i] = d;
-    }
-  const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, lds, 1) / (float)D + eps);
-  T *yr = y + row * (long)D;
-#pragma unroll
-  for (int c = 0; c < E / V; ++c) {
-    const int col = (c * TPR + t) * V;
-    if (col < D) {
-      float o[V], p[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = v[c * V + i] * rstd;
-      if (w) {
-        load_param<T, V>(w, param_f32, col, p);
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] *= p[i];
-      }
-      if (b) {
-        load_param<T, V>(b, param_f32, col, p);
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] += p[i];
-      }
-      store_vec<T, V>(yr + col, o);
-    }
+  for (int e = 0; e < R::EX; ++e) {
+    const float d = v[e] - mean;
+    if (R::holds(e, t, D)) q = fmaf(d, d, q);
+    v[e] = d;
   }
+  const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, lds, 1) / (float)D + eps);
+#pragma unroll
+  for (int e = 0; e < R::EX; ++e) v[e] *= rstd;
+  if (w) {
+    R::param(w, param_f32, t, D, p);
+#pragma unroll
+    for (int e = 0; e < R::EX; ++e) v[e] *= p[e];
+  }
+  if (b) {
+    R::param(b, param_f32, t, D, p);
+#pragma unroll
+    for (int e = 0; e < R::EX; ++e) v[e] += p[e];
+  }
+  R::store(y + row * (long)D, t, D, v);
   if (stats && t == 0) {
     stats[row] = mean;
     stats[rows + row] = rstd;
@@ -106,21 +154,22 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_kernel(
 }
 
 // part: gridDim.x rows of 2 D floats (weight gradient, bias gradient), or NULL when neither is wanted.
-template <typename T, int TPR, int E, int V>
+template <typename T, int TPR, int E, bool ALIGNED>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_backward_kernel(
     const T *__restrict__ dy, long lddy, const T *__restrict__ x, long ldx, const void *__restrict__ w, int param_f32,
     const float *__restrict__ stats, long rows, int D, T *__restrict__ dx, float *__restrict__ part) {
+  typedef Row<T, TPR, E, ALIGNED> R;
   constexpr int RPB = TPR == 64 ? 4 : 1;
   constexpr int JOIN = TPR == 64 ? 64 * 4 * 8 : 1;
   __shared__ float lds[4 * (TPR / 64)];
   __shared__ float join[JOIN];
   const int t = TPR == 64 ? threadIdx.x & 63 : threadIdx.x;
   const int sub = TPR == 64 ? threadIdx.x >> 6 : 0;
-  float dw[E], db[E];
+  float dw[R::EX], db[R::EX];
 #pragma unroll
-  for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
+  for (int e = 0; e < R::EX; ++e) dw[e] = db[e] = 0.0f;
   int slot = 0;
-  Row<T, TPR, E, V> rg, rx;  // the next row is under way while this one is worked on
+  R rg, rx;  // the next row is under way while this one is worked on
   float rmean, rrstd;
   auto fetch = [&](long row) {
     rg.load(dy + row * lddy, t, D);
@@ -131,7 +180,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_backward_
   const long first = (long)blockIdx.x * RPB + sub;
   if (first < rows) fetch(first);
   for (long row = first; row < rows; row += (long)gridDim.x * RPB) {
-    float g[E], h[E];
+    float g[R::EX], h[R::EX];
     rg.get(t, D, g);
     rx.get(t, D, h);
     const float mean = rmean, rstd = rrstd;
@@ -139,66 +188,55 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void bk_layer_norm_backward_
     if (next < rows) fetch(next);
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-    for (int c = 0; c < E / V; ++c) {
-      const int col = (c * TPR + t) * V;
-      if (col < D) {
-        float p[V];
-        if (w) load_param<T, V>(w, param_f32, col, p);
+    for (int e = 0; e < R::EX; ++e) {
+      h[e] = R::holds(e, t, D) ? (h[e] - mean) * rstd : 0.0f;
+      dw[e] = fmaf(g[e], h[e], dw[e]);
+      db[e] += g[e];
+    }
+    if (w) {
+      float p[R::EX];
+      R::param(w, param_f32, t, D, p);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int e = c * V + i;
-          h[e] = (h[e] - mean) * rstd;
-          dw[e] = fmaf(g[e], h[e], dw[e]);
-          db[e] += g[e];
-          if (w) g[e] *= p[i];
-          s0 += g[e];
-          s1 = fmaf(g[e], h[e], s1);
-        }
-      }
+      for (int e = 0; e < R::EX; ++e) g[e] *= p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < R::EX; ++e) {
+      s0 += g[e];
+      s1 = fmaf(g[e], h[e], s1);
     }
     s0 = row_sum<TPR>(s0, lds, 2 * slot) / (float)D;
     s1 = row_sum<TPR>(s1, lds, 2 * slot + 1) / (float)D;
     slot ^= 1;
-    T *dr = dx + row * (long)D;
 #pragma unroll
-    for (int c = 0; c < E / V; ++c) {
-      const int col = (c * TPR + t) * V;
-      if (col < D) {
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = rstd * (g[c * V + i] - s0 - h[c * V + i] * s1);
-        store_vec<T, V>(dr + col, o);
-      }
-    }
+    for (int e = 0; e < R::EX; ++e) g[e] = rstd * (g[e] - s0 - h[e] * s1);
+    R::store(dx + row * (long)D, t, D, g);
   }
   if (!part) return;
   float *pw = part + (long)blockIdx.x * 2 * D, *pb = pw + D;
   if constexpr (TPR == 64) {  // the four waves of the workgroup hold the same columns: join them, 8 at a time
-    constexpr int G = E < 8 ? E : 8;
+    constexpr int G = 8, N = (R::EX + G - 1) / G;
 #pragma unroll
-    for (int k = 0; k < 2 * E / G; ++k) {
-      const int e0 = (k % (E / G)) * G;
+    for (int k = 0; k < 2 * N; ++k) {
+      const int e0 = (k % N) * G;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < G; ++i) join[(sub * G + i) * 64 + t] = k < E / G ? dw[e0 + i] : db[e0 + i];
+      for (int i = 0; i < G; ++i)
+        if (e0 + i < R::EX) join[(sub * G + i) * 64 + t] = k < N ? dw[e0 + i < R::EX ? e0 + i : 0] : db[e0 + i < R::EX ? e0 + i : 0];
       __syncthreads();
       for (int j = threadIdx.x; j < G * 64; j += 256) {
         const int i = j >> 6, l = j & 63, e = e0 + i;
-        const int col = ((e / V) * 64 + l) * V + e % V;
-        if (col < D)
-          (k < E / G ? pw : pb)[col] = join[i * 64 + l] + join[(G + i) * 64 + l] + join[(2 * G + i) * 64 + l] +
-                                       join[(3 * G + i) * 64 + l];
+        if (e < R::EX && R::holds(e, l, D))
+          (k < N ? pw : pb)[R::column(e, l, D)] = join[i * 64 + l] + join[(G + i) * 64 + l] + join[(2 * G + i) * 64 + l] +
+                                                  join[(3 * G + i) * 64 + l];
       }
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int col = ((e / V) * TPR + t) * V + e % V;
-      if (col < D) {
-        pw[col] = dw[e];
-        pb[col] = db[e];
+    for (int e = 0; e < R::EX; ++e)
+      if (R::holds(e, t, D)) {
+        pw[R::column(e, t, D)] = dw[e];
+        pb[R::column(e, t, D)] = db[e];
       }
-    }
   }
 }
 
@@ -246,7 +284,7 @@ extern "C" void bkcore_internal_sum_parts(const float *part, int64_t parts, int6
     else if (D <= 2048) LAUNCH(64, 32);         \
     else if (D <= 4096) LAUNCH(256, 16);        \
     else if (D <= 8192) LAUNCH(256, 32);        \
-    else LAUNCH(1024, 16);                      \
+    else LAUNCH(512, 32);                      \
   } while (0)
 
 extern "C" int bkcore_layer_norm(const void *x, int64_t ldx, int dtype, const void *weight, const void *bias,
@@ -266,8 +304,8 @@ extern "C" int bkcore_layer_norm(const void *x, int64_t ldx, int dtype, const vo
                      (int)D, (T *)y, stats)
 #define BK_LN(TPR, E)                                           \
   do {                                                          \
-    if (vec) BK_LN_V(TPR, E, (int)(16 / sizeof(T)));            \
-    else BK_LN_V(TPR, E, 1);                                    \
+    if (vec) BK_LN_V(TPR, E, true);                             \
+    else BK_LN_V(TPR, E, false);                                \
   } while (0)
   BK_WITH_TYPE(dtype, BK_NORM_SHAPES(BK_LN));
 #undef BK_LN
@@ -301,8 +339,8 @@ extern "C" int bkcore_layer_norm_backward(const void *dy, int64_t lddy, const vo
                      (const T *)dy, (long)lddy, (const T *)x, (long)ldx, weight, pf, stats, (long)rows, (int)D, (T *)dx, part)
 #define BK_LN(TPR, E)                                           \
   do {                                                          \
-    if (vec) BK_LN_V(TPR, E, (int)(16 / sizeof(T)));            \
-    else BK_LN_V(TPR, E, 1);                                    \
+    if (vec) BK_LN_V(TPR, E, true);                             \
+    else BK_LN_V(TPR, E, false);                                \
   } while (0)
   BK_WITH_TYPE(dtype, BK_NORM_SHAPES(BK_LN));
 #undef BK_LN

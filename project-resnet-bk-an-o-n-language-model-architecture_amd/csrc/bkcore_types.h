@@ -65,6 +65,24 @@ struct RawVec {
     for (int i = 0; i < V; ++i) v[i] = in ? (float)w[i] : 0.0f;
   }
 };
+// V elements at an address that is aligned to one element only (the hardware takes wide accesses at any address).
+template <typename T, int V>
+struct LooseVec {
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  typedef vec_t loose_t __attribute__((aligned(sizeof(T))));
+  vec_t w;
+  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *reinterpret_cast<const loose_t *>(p); }
+  __device__ __forceinline__ void get(bool in, float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = in ? (float)w[i] : 0.0f;
+  }
+  static __device__ __forceinline__ void store(T *__restrict__ p, const float (&v)[V]) {
+    vec_t w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = (T)v[i];
+    *reinterpret_cast<loose_t *>(p) = w;
+  }
+};
 template <typename T>
 struct RawVec<T, 1> {
   T w;
