@@ -32,13 +32,27 @@ __device__ __forceinline__ int row_length(const int *lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : n;
 }
 
+template <typename T, int V, bool AL>
+__device__ __forceinline__ void load_piece(const T *__restrict__ p, float (&v)[V]) {
+  Piece<T, V, AL> r;
+  r.load(p);
+  r.get(true, v);
+}
+
+// First channel of the i-th piece: the last one reaches back into its neighbour where V does not divide the channels (both
+// compute and write the same values there).
+template <int V>
+__device__ __forceinline__ int piece_channel(int i, int C) {
+  return V == 1 || (i + 1) * V <= C ? i * V : C - V;
+}
+
 // x_t of sequence b for V channels from c: the carried state for t < 0, zero where there is none or behind the length.
-template <typename T, int K, int V>
+template <typename T, int K, int V, bool AL>
 __device__ __forceinline__ void input_at(const ConvArgs &a, int b, long t, int len, int c, float (&v)[V]) {
   if (t >= 0 && t < len) {
-    load_vec<T, V>((const T *)a.x + b * a.xb + t * a.xt + c, v);
+    load_piece<T, V, AL>((const T *)a.x + b * a.xb + t * a.xt + c, v);
   } else if (t < 0 && a.init) {
-    load_vec<T, V>((const T *)a.init + ((long)b * (K - 1) + (t + K - 1)) * a.C + c, v);
+    load_piece<T, V, AL>((const T *)a.init + ((long)b * (K - 1) + (t + K - 1)) * a.C + c, v);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = 0.0f;
@@ -46,10 +60,10 @@ __device__ __forceinline__ void input_at(const ConvArgs &a, int b, long t, int l
 }
 
 // The taps of V channels are V K neighbouring values; in float32 and aligned they come as 16-byte loads.
-template <typename T, int K, int V>
+template <typename T, int K, int V, bool AL>
 __device__ __forceinline__ void load_taps(const ConvArgs &a, int c, float (&w)[K][V], float (&bias)[V]) {
   float flat[V * K];
-  if (V > 1 && a.param_vec) {
+  if (V > 1 && AL && a.param_vec) {
     const f32x4 *p = reinterpret_cast<const f32x4 *>((const float *)a.w + (long)c * K);
 #pragma unroll
     for (int j = 0; j < V * K / 4; ++j) {
@@ -69,24 +83,24 @@ __device__ __forceinline__ void load_taps(const ConvArgs &a, int c, float (&w)[K
   if (a.bias) load_param<T, V>(a.bias, a.param_f32, c, bias);
 }
 
-template <typename T, int K, int V>
+template <typename T, int K, int V, bool AL>
 __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int nvec) {
   const long id = (long)blockIdx.x * 256 + threadIdx.x;
   if (id >= (long)a.B * nseg * nvec) return;
-  const int c = (int)(id % nvec) * V;
+  const int c = piece_channel<V>((int)(id % nvec), a.C);
   const long r = id / nvec;
   const int seg = (int)(r % nseg), b = (int)(r / nseg);
   const int len = row_length(a.lengths, b, a.L);
   const int t0 = seg * FWD_TL, t1 = t0 + FWD_TL < a.L ? t0 + FWD_TL : a.L;
   if (t0 < a.L) {
     const T *x = (const T *)a.x + b * a.xb + c;
-    RawVec<T, V> raw[FWD_TL];  // all of the stretch is under way before its first position is worked on
+    Piece<T, V, AL> raw[FWD_TL];  // all of the stretch is under way before its first position is worked on
 #pragma unroll
     for (int j = 0; j < FWD_TL; ++j) raw[j].load(x + (long)(t0 + j < a.L ? t0 + j : a.L - 1) * a.xt);
     float w[K][V], bias[V], h[K][V];
-    load_taps<T, K, V>(a, c, w, bias);
+    load_taps<T, K, V, AL>(a, c, w, bias);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) input_at<T, K, V>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+    for (int k = 0; k < K - 1; ++k) input_at<T, K, V, AL>(a, b, t0 - (K - 1) + k, len, c, h[k]);
     T *y = (T *)a.y + ((long)b * a.L) * a.C + c;
 #pragma unroll
     for (int j = 0; j < FWD_TL; ++j) {
@@ -101,7 +115,7 @@ __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int 
         if (a.silu) s = s * sigmoid(s);
         o[i] = t < len ? s : 0.0f;
       }
-      if (t < t1) store_vec<T, V>(y + (long)t * a.C, o);
+      if (t < t1) Piece<T, V, AL>::store(y + (long)t * a.C, o);
 #pragma unroll
       for (int k = 0; k < K - 1; ++k)
 #pragma unroll
@@ -112,23 +126,23 @@ __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int 
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
       float v[V];
-      input_at<T, K, V>(a, b, (long)len - (K - 1) + j, len, c, v);
-      store_vec<T, V>((T *)a.final_state + ((long)b * (K - 1) + j) * a.C + c, v);
+      input_at<T, K, V, AL>(a, b, (long)len - (K - 1) + j, len, c, v);
+      Piece<T, V, AL>::store((T *)a.final_state + ((long)b * (K - 1) + j) * a.C + c, v);
     }
   }
 }
 
 // One workgroup: 32 channel vectors x 8 stretches of 32 positions of one sequence.  part: one row of (K + 1) C floats
 // per (sequence, workgroup along time): the weights' sums (C, K), then the bias'.
-template <typename T, int K, int V>
-__global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(ConvArgs a, int nblk, int cblk) {
+template <typename T, int K, int V, bool AL>
+__global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(ConvArgs a, int nblk, int cblk, int nvec) {
   __shared__ float join[BWD_SEGS][BWD_CH][V + 1];
   const int cv = threadIdx.x % BWD_CH, sg = threadIdx.x / BWD_CH;
   const int cb = blockIdx.x % cblk;
   const long stretch = blockIdx.x / cblk;  // sequence and workgroup along time
   const int b = (int)(stretch / nblk), tb = (int)(stretch % nblk);
-  const int c = (cb * BWD_CH + cv) * V;
-  const bool live = c < a.C;
+  const bool live = cb * BWD_CH + cv < nvec;
+  const int c = piece_channel<V>(cb * BWD_CH + cv, a.C);
   const int len = row_length(a.lengths, b, a.L);
   float dw[K][V], db[V];
 #pragma unroll
@@ -141,19 +155,19 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
   const long t1 = t0 + BWD_TL < a.L ? t0 + BWD_TL : a.L;
   if (live && t0 < a.L) {
     float w[K][V], bias[V], h[K][V], g[K][V];  // h: x_{t-K+1..t};  g: g_{t-K+1..t}
-    load_taps<T, K, V>(a, c, w, bias);
+    load_taps<T, K, V, AL>(a, c, w, bias);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) input_at<T, K, V>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+    for (int k = 0; k < K - 1; ++k) input_at<T, K, V, AL>(a, b, t0 - (K - 1) + k, len, c, h[k]);
     const T *dy = (const T *)a.dy + b * a.dyb + c;
     T *dx = (T *)a.dx + (long)b * a.L * a.C + c;
     // dx of position t - K + 1 is complete once g_t is known; the first stretch also gives the carried state's gradient
     const T *x = (const T *)a.x + b * a.xb + c;
     struct Block {
-      RawVec<T, V> x[BWD_UNDER], g[BWD_UNDER];
+      Piece<T, V, AL> x[BWD_UNDER], g[BWD_UNDER];
     } cur, next;
     auto fetch = [&](long from) {
 #pragma unroll
@@ -208,14 +222,14 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
         const long j = p - ((long)len - (K - 1));  // its place in the final state
         if (a.dfinal && j >= 0 && p < len) {
           float f[V];
-          load_vec<T, V>((const T *)a.dfinal + ((long)b * (K - 1) + j) * a.C + c, f);
+          load_piece<T, V, AL>((const T *)a.dfinal + ((long)b * (K - 1) + j) * a.C + c, f);
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] += f[i];
         }
         if (p >= t0)
-          store_vec<T, V>(dx + p * a.C, o);
+          Piece<T, V, AL>::store(dx + p * a.C, o);
         else
-          store_vec<T, V>((T *)a.dinit + ((long)b * (K - 1) + (p + K - 1)) * a.C + c, o);
+          Piece<T, V, AL>::store((T *)a.dinit + ((long)b * (K - 1) + (p + K - 1)) * a.C + c, o);
       }
 #pragma unroll
       for (int k = 0; k < K - 1; ++k)
@@ -236,8 +250,8 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
     for (int i = 0; i < V; ++i) join[sg][cv][i] = k < K ? dw[k < K ? k : 0][i] : db[i];
     __syncthreads();
     for (int j = threadIdx.x; j < BWD_CH * V; j += BWD_CH * BWD_SEGS) {
-      const int col = cb * BWD_CH * V + j;
-      if (col < a.C) {
+      if (cb * BWD_CH + j / V < nvec) {
+        const int col = piece_channel<V>(cb * BWD_CH + j / V, a.C) + j % V;
         float s = 0.0f;
 #pragma unroll
         for (int q = 0; q < BWD_SEGS; ++q) s += join[q][j / V][j % V];
@@ -248,17 +262,17 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
 }
 
 // One token: the window is the state and the new input; the state moves on by one position in place.
-template <typename T, int K, int V>
+template <typename T, int K, int V, bool AL>
 __global__ __launch_bounds__(256) void bk_conv_step_kernel(ConvArgs a, T *__restrict__ state, int nvec) {
   const long id = (long)blockIdx.x * 256 + threadIdx.x;
   if (id >= (long)a.B * nvec) return;
-  const int c = (int)(id % nvec) * V, b = (int)(id / nvec);
+  const int c = piece_channel<V>((int)(id % nvec), a.C), b = (int)(id / nvec);
   float w[K][V], bias[V], h[K][V];
-  load_taps<T, K, V>(a, c, w, bias);
+  load_taps<T, K, V, AL>(a, c, w, bias);
   T *st = state + (long)b * (K - 1) * a.C + c;
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) load_vec<T, V>(st + (long)k * a.C, h[k]);
-  load_vec<T, V>((const T *)a.x + b * a.xb + c, h[K - 1]);
+  for (int k = 0; k < K - 1; ++k) load_piece<T, V, AL>(st + (long)k * a.C, h[k]);
+  load_piece<T, V, AL>((const T *)a.x + b * a.xb + c, h[K - 1]);
   float o[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -268,8 +282,8 @@ __global__ __launch_bounds__(256) void bk_conv_step_kernel(ConvArgs a, T *__rest
     o[i] = a.silu ? s * sigmoid(s) : s;
   }
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) store_vec<T, V>(st + (long)k * a.C, h[k + 1]);
-  store_vec<T, V>((T *)a.y + (long)b * a.C + c, o);
+  for (int k = 0; k < K - 1; ++k) Piece<T, V, AL>::store(st + (long)k * a.C, h[k + 1]);
+  Piece<T, V, AL>::store((T *)a.y + (long)b * a.C + c, o);
 }
 
 int check(int dtype, int param_dtype, int64_t B, int64_t L, int64_t C, int64_t K) {
@@ -283,11 +297,18 @@ inline int64_t backward_blocks(int64_t L) { return (L + BWD_TL * BWD_SEGS - 1) /
 
 }  // namespace
 
-#define BK_CONV_K(K, LAUNCH, V)             \
+#define BK_CONV_K(K, LAUNCH, V, AL)         \
   do {                                      \
-    if ((K) == 2) LAUNCH(2, V);             \
-    else if ((K) == 3) LAUNCH(3, V);        \
-    else LAUNCH(4, V);                      \
+    if ((K) == 2) LAUNCH(2, V, AL);         \
+    else if ((K) == 3) LAUNCH(3, V, AL);    \
+    else LAUNCH(4, V, AL);                  \
+  } while (0)
+// 16-byte pieces at 16-byte addresses, at any addresses, or single channels where there are fewer than a piece
+#define BK_CONV_ANY(K, LAUNCH, V, PIECES)                             \
+  do {                                                                \
+    if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, LAUNCH, V, true));      \
+    else if (PIECES) BK_WITH_TYPE(dtype, BK_CONV_K(K, LAUNCH, V, false)); \
+    else BK_WITH_TYPE(dtype, BK_CONV_K(K, LAUNCH, 1, false));         \
   } while (0)
 
 extern "C" int bkcore_causal_conv(const void *x, int64_t x_batch, int64_t x_time, int dtype, const void *weight,
@@ -305,14 +326,13 @@ extern "C" int bkcore_causal_conv(const void *x, int64_t x_batch, int64_t x_time
   a.x = x; a.w = weight; a.bias = bias; a.init = initial_state; a.y = y; a.final_state = final_state;
   a.lengths = lengths; a.xb = x_batch; a.xt = x_time; a.B = (int)B; a.L = (int)L; a.C = (int)C;
   a.param_f32 = param_dtype == BKCORE_F32; a.param_vec = a.param_f32 && aligned16(weight); a.silu = silu != 0;
-  const int64_t nseg = L > 0 ? (L + FWD_TL - 1) / FWD_TL : 1, nvec = vec ? C / v : C;
+  const int64_t nseg = L > 0 ? (L + FWD_TL - 1) / FWD_TL : 1, nvec = C >= v ? (C + v - 1) / v : C;
   const int64_t blocks = (B * nseg * nvec + 255) / 256;
   if (blocks > 2147483647LL) return BKCORE_EINVAL;
-#define BK_CONV(K_, V_)                                                                                            \
-  hipLaunchKernelGGL((bk_conv_kernel<T, K_, V_>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, (int)nseg, \
+#define BK_CONV(K_, V_, AL_)                                                                                            \
+  hipLaunchKernelGGL((bk_conv_kernel<T, K_, V_, AL_>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, (int)nseg, \
                      (int)nvec)
-  if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, (int)(16 / sizeof(T))));
-  else BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, 1));
+  BK_CONV_ANY(K, BK_CONV, (int)(16 / sizeof(T)), C >= v);
 #undef BK_CONV
   return launch_status();
 }
@@ -344,13 +364,12 @@ extern "C" int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int
   a.dx = dx; a.dinit = grad_initial_state; a.part = grad_params ? (float *)workspace : nullptr; a.lengths = lengths;
   a.xb = x_batch; a.xt = x_time; a.dyb = dy_batch; a.dyt = dy_time; a.B = (int)B; a.L = (int)L; a.C = (int)C;
   a.param_f32 = param_dtype == BKCORE_F32; a.param_vec = a.param_f32 && aligned16(weight); a.silu = silu != 0;
-  const int64_t nblk = backward_blocks(L), nvec = vec ? C / v : C, cblk = (nvec + BWD_CH - 1) / BWD_CH;
+  const int64_t nblk = backward_blocks(L), nvec = C >= v ? (C + v - 1) / v : C, cblk = (nvec + BWD_CH - 1) / BWD_CH;
   if (B * nblk * cblk > 2147483647LL) return BKCORE_EINVAL;
-#define BK_CONV(K_, V_)                                                                                              \
-  hipLaunchKernelGGL((bk_conv_backward_kernel<T, K_, V_>), dim3((unsigned)(B * nblk * cblk)), dim3(BWD_CH * BWD_SEGS), \
-                     0, (hipStream_t)stream, a, (int)nblk, (int)cblk)
-  if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, (int)(16 / sizeof(T))));
-  else BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, 1));
+#define BK_CONV(K_, V_, AL_)                                                                                              \
+  hipLaunchKernelGGL((bk_conv_backward_kernel<T, K_, V_, AL_>), dim3((unsigned)(B * nblk * cblk)), dim3(BWD_CH * BWD_SEGS), \
+                     0, (hipStream_t)stream, a, (int)nblk, (int)cblk, (int)nvec)
+  BK_CONV_ANY(K, BK_CONV, (int)(16 / sizeof(T)), C >= v);
 #undef BK_CONV
   if (grad_params) bkcore_internal_sum_parts((const float *)workspace, B * nblk, (K + 1) * C, grad_params, stream);
   return launch_status();
@@ -368,13 +387,13 @@ extern "C" int bkcore_causal_conv_step(const void *x, int64_t x_batch, int dtype
   ConvArgs a{};
   a.x = x; a.w = weight; a.bias = bias; a.y = y; a.xb = x_batch; a.B = (int)B; a.L = 1; a.C = (int)C;
   a.param_f32 = param_dtype == BKCORE_F32; a.param_vec = a.param_f32 && aligned16(weight); a.silu = silu != 0;
-  const int64_t nvec = vec ? C / v : C, blocks = (B * nvec + 255) / 256;
+  // whole pieces only: two threads on one channel would race on the state
+  const int64_t nvec = C % v == 0 ? C / v : C, blocks = (B * nvec + 255) / 256;
   if (blocks > 2147483647LL) return BKCORE_EINVAL;
-#define BK_CONV(K_, V_)                                                                                              \
-  hipLaunchKernelGGL((bk_conv_step_kernel<T, K_, V_>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, \
+#define BK_CONV(K_, V_, AL_)                                                                                              \
+  hipLaunchKernelGGL((bk_conv_step_kernel<T, K_, V_, AL_>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, \
                      (T *)state, (int)nvec)
-  if (vec) BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, (int)(16 / sizeof(T))));
-  else BK_WITH_TYPE(dtype, BK_CONV_K(K, BK_CONV, 1));
+  BK_CONV_ANY(K, BK_CONV, (int)(16 / sizeof(T)), C % v == 0);
 #undef BK_CONV
   return launch_status();
 }

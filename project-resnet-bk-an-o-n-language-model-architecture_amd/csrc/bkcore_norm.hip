@@ -35,8 +35,8 @@ __device__ __forceinline__ float row_sum(float x, float *lds, int slot) {
 template <typename T, int TPR, int E, bool ALIGNED>
 struct Row {
   static constexpr int V = 16 / (int)sizeof(T), EX = ALIGNED ? E : E + 1;
-  LooseVec<T, V> r[E / V];
-  RawVec<T, V> ra[E / V];
+  typedef Piece<T, V, ALIGNED> P;
+  P r[E / V];
   T last;
   static __device__ __forceinline__ int whole(int D) { return ALIGNED ? D : D / V * V; }
   static __device__ __forceinline__ int column(int e, int t, int D) {
@@ -51,8 +51,7 @@ struct Row {
 #pragma unroll
       for (int c = 0; c < E / V; ++c) {
         const int col = (c * TPR + t) * V;
-        if constexpr (ALIGNED) ra[c].load(p + (col < Dv ? col : 0));
-        else r[c].load(p + (col < Dv ? col : 0));
+        r[c].load(p + (col < Dv ? col : 0));
       }
     }
     if constexpr (!ALIGNED) last = p[t < D - Dv ? Dv + t : 0];
@@ -61,8 +60,7 @@ struct Row {
 #pragma unroll
     for (int c = 0; c < E / V; ++c) {
       float w[V];
-      if constexpr (ALIGNED) ra[c].get(holds(c * V, t, D), w);
-      else r[c].get(holds(c * V, t, D), w);
+      r[c].get(holds(c * V, t, D), w);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[c * V + i] = w[i];
     }
@@ -77,8 +75,7 @@ struct Row {
         float w[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) w[i] = o[c * V + i];
-        if constexpr (ALIGNED) store_vec<T, V>(p + col, w);
-        else LooseVec<T, V>::store(p + col, w);
+        P::store(p + col, w);
       }
     }
     if constexpr (!ALIGNED) {

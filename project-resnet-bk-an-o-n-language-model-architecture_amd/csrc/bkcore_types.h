@@ -53,43 +53,6 @@ __device__ __forceinline__ void load_vec(const T *__restrict__ p, float (&v)[V])
   }
 }
 
-// The same in two steps, so that several loads are under way before the first is waited for: a load converted where it
-// is issued, or issued under a condition, is waited for at once.
-template <typename T, int V>
-struct RawVec {
-  typedef T vec_t __attribute__((ext_vector_type(V)));
-  vec_t w;
-  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *reinterpret_cast<const vec_t *>(p); }
-  __device__ __forceinline__ void get(bool in, float (&v)[V]) const {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = in ? (float)w[i] : 0.0f;
-  }
-};
-// V elements at an address that is aligned to one element only (the hardware takes wide accesses at any address).
-template <typename T, int V>
-struct LooseVec {
-  typedef T vec_t __attribute__((ext_vector_type(V)));
-  typedef vec_t loose_t __attribute__((aligned(sizeof(T))));
-  vec_t w;
-  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *reinterpret_cast<const loose_t *>(p); }
-  __device__ __forceinline__ void get(bool in, float (&v)[V]) const {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = in ? (float)w[i] : 0.0f;
-  }
-  static __device__ __forceinline__ void store(T *__restrict__ p, const float (&v)[V]) {
-    vec_t w;
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = (T)v[i];
-    *reinterpret_cast<loose_t *>(p) = w;
-  }
-};
-template <typename T>
-struct RawVec<T, 1> {
-  T w;
-  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *p; }
-  __device__ __forceinline__ void get(bool in, float (&v)[1]) const { v[0] = in ? (float)w : 0.0f; }
-};
-
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T *__restrict__ p, const float (&v)[V]) {
   if constexpr (V == 1) {
@@ -157,6 +120,34 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * LOG2E));
 }
+
+// V neighbouring elements of a row, at 16-byte (ALIGNED) or at any addresses: held raw until they are
+// used, so that several loads are under way before the first is waited for (a load converted where it is issued, or issued
+// under a condition, is waited for at once).
+template <typename T, int V, bool ALIGNED>
+struct Piece {
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  typedef vec_t mem_t __attribute__((aligned(ALIGNED ? sizeof(T) * V : sizeof(T))));
+  vec_t w;
+  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *reinterpret_cast<const mem_t *>(p); }
+  __device__ __forceinline__ void get(bool in, float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = in ? (float)w[i] : 0.0f;
+  }
+  static __device__ __forceinline__ void store(T *__restrict__ p, const float (&v)[V]) {
+    vec_t w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = (T)v[i];
+    *reinterpret_cast<mem_t *>(p) = w;
+  }
+};
+template <typename T, bool ALIGNED>
+struct Piece<T, 1, ALIGNED> {
+  T w;
+  __device__ __forceinline__ void load(const T *__restrict__ p) { w = *p; }
+  __device__ __forceinline__ void get(bool in, float (&v)[1]) const { v[0] = in ? (float)w : 0.0f; }
+  static __device__ __forceinline__ void store(T *__restrict__ p, const float (&v)[1]) { *p = (T)v[0]; }
+};
 
 }  // namespace bk
 
