@@ -71,4 +71,6 @@ def lengths_arg(what: str, lengths: torch.Tensor | None, x: torch.Tensor, batch:
     return lengths.clamp(0, longest).to(torch.int32)
 
 
-stream = torch._C._cuda_getCurrentRawStream     # of a device index: the handle alone, without a Stream object around it
+def stream(index: int) -> int:
+    """The current stream's handle on a device, without a Stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(index)

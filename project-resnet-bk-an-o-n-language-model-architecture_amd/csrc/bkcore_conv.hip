@@ -3,17 +3,18 @@
 //   pre_t = bias + sum_k w_k x_{t-K+1+k},  y_t = pre_t or silu(pre_t);  x at t < 0 is the carried state, or zero
 //   g_t = dy_t act'(pre_t);  dx_t = sum_k w_k g_{t+K-1-k};  dw_k = sum g_t x_{t-K+1+k};  db = sum g_t
 // Positions at or behind a sequence's length are padding: they are never read, y and dx there are zero.
-// HBM-bound: 2 e bytes an element forward, 3 e backward.  A thread holds V neighbouring channels (one 16-byte access a
-// position) and walks TL positions with the last K - 1 inputs in registers; only the K - 1 positions in front of its
-// stretch are read twice, from cache.  Arithmetic and sums are float32.
+// HBM-bound: 2 e bytes an element forward, 3 e backward (8 x 2048 x 1024 bf16: 18.5 us = 3.6 TB/s, and 31.9 + 4 us =
+// 2.8 TB/s).  A thread holds V neighbouring channels (16 bytes a position forward, 4 channels backward, where five sums and
+// two windows a channel take the registers) and walks a stretch of positions with the last K - 1 inputs in registers; only
+// the K - 1 positions in front of its stretch are read twice, from cache.  Arithmetic and sums are float32.
 #include "bkcore_types.h"
 
 namespace {
 using namespace bk;
 
-constexpr int FWD_TL = 16;  // positions a thread walks forward: 3 of 19 reads are repeated
-constexpr int BWD_TL = 32;  // ... and backward
-constexpr int BWD_UNDER = 5; // positions of a block; the next block is under way while one is worked on
+constexpr int FWD_TL = 9;   // positions a thread walks forward; stretches a power of two apart meet on the same memory channels
+                            // (8 x 2048 x 1024 bf16: 18.5 us at 9, 20.4 at 8, 19.7 at 16)
+constexpr int BWD_TL = 16;  // ... and backward (31.9 us there and 12.8 at 2 x 300 x 256; 32: 30.0 and 22.1)
 constexpr int BWD_SEGS = 8; // stretches of one workgroup, joined before the partial sums are written
 constexpr int BWD_CH = 32;  // channel vectors of one workgroup
 
@@ -59,6 +60,31 @@ __device__ __forceinline__ void input_at(const ConvArgs &a, int b, long t, int l
   }
 }
 
+// The K - 1 inputs in front of position t0, all under way together: positions, or the carried state in front of the first.
+template <typename T, int K, int V, bool AL>
+struct Halo {
+  Piece<T, V, AL> r[K - 1];
+  __device__ __forceinline__ void load(const T *__restrict__ x, long step, long t0, int L) {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      const long t = t0 - (K - 1) + k;
+      r[k].load(x + (t < 0 ? 0 : t < L ? t : L - 1) * step);
+    }
+  }
+  __device__ __forceinline__ void get(const ConvArgs &a, int b, long t0, int len, int c, float (&h)[K][V]) const {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      const long t = t0 - (K - 1) + k;
+      r[k].get(t >= 0 && t < len, h[k]);
+    }
+    if (t0 == 0 && a.init) {  // stretches are longer than the window: only the first one reaches in front of the sequence
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+        load_piece<T, V, AL>((const T *)a.init + ((long)b * (K - 1) + k) * a.C + c, h[k]);
+    }
+  }
+};
+
 // The taps of V channels are V K neighbouring values; in float32 and aligned they come as 16-byte loads.
 template <typename T, int K, int V, bool AL>
 __device__ __forceinline__ void load_taps(const ConvArgs &a, int c, float (&w)[K][V], float (&bias)[V]) {
@@ -97,10 +123,11 @@ __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int 
     Piece<T, V, AL> raw[FWD_TL];  // all of the stretch is under way before its first position is worked on
 #pragma unroll
     for (int j = 0; j < FWD_TL; ++j) raw[j].load(x + (long)(t0 + j < a.L ? t0 + j : a.L - 1) * a.xt);
+    Halo<T, K, V, AL> halo;
+    halo.load(x, a.xt, t0, a.L);
     float w[K][V], bias[V], h[K][V];
     load_taps<T, K, V, AL>(a, c, w, bias);
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) input_at<T, K, V, AL>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+    halo.get(a, b, t0, len, c, h);
     T *y = (T *)a.y + ((long)b * a.L) * a.C + c;
 #pragma unroll
     for (int j = 0; j < FWD_TL; ++j) {
@@ -132,7 +159,7 @@ __global__ __launch_bounds__(256) void bk_conv_kernel(ConvArgs a, int nseg, int 
   }
 }
 
-// One workgroup: 32 channel vectors x 8 stretches of 32 positions of one sequence.  part: one row of (K + 1) C floats
+// One workgroup: 32 pieces of channels x 8 stretches of positions of one sequence.  part: one row of (K + 1) C floats
 // per (sequence, workgroup along time): the weights' sums (C, K), then the bias'.
 template <typename T, int K, int V, bool AL>
 __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(ConvArgs a, int nblk, int cblk, int nvec) {
@@ -155,34 +182,38 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
   const long t1 = t0 + BWD_TL < a.L ? t0 + BWD_TL : a.L;
   if (live && t0 < a.L) {
     float w[K][V], bias[V], h[K][V], g[K][V];  // h: x_{t-K+1..t};  g: g_{t-K+1..t}
-    load_taps<T, K, V, AL>(a, c, w, bias);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) input_at<T, K, V, AL>(a, b, t0 - (K - 1) + k, len, c, h[k]);
+    Halo<T, K, V, AL> halo;
+    halo.load((const T *)a.x + b * a.xb + c, a.xt, t0, a.L);
     const T *dy = (const T *)a.dy + b * a.dyb + c;
     T *dx = (T *)a.dx + (long)b * a.L * a.C + c;
     // dx of position t - K + 1 is complete once g_t is known; the first stretch also gives the carried state's gradient
     const T *x = (const T *)a.x + b * a.xb + c;
+    // Positions of a block, the next one under way while this one is worked on; a multiple of K, so that the windows h and g
+    // are back in the same registers behind it.
+    constexpr int UNDER = K == 3 ? 6 : 4;
     struct Block {
-      Piece<T, V, AL> x[BWD_UNDER], g[BWD_UNDER];
+      Piece<T, V, AL> x[UNDER], g[UNDER];
     } cur, next;
     auto fetch = [&](long from) {
 #pragma unroll
-      for (int j = 0; j < BWD_UNDER; ++j) {
+      for (int j = 0; j < UNDER; ++j) {
         const long t = from + j < a.L ? from + j : a.L - 1;
         next.x[j].load(x + t * a.xt);
         next.g[j].load(dy + t * a.dyt);
       }
     };
     fetch(t0);
-    for (long tb0 = t0; tb0 < t1 + K - 1; tb0 += BWD_UNDER) {
-    cur = next;
-    if (tb0 + BWD_UNDER < t1 + K - 1) fetch(tb0 + BWD_UNDER);
+    load_taps<T, K, V, AL>(a, c, w, bias);
+    halo.get(a, b, t0, len, c, h);
 #pragma unroll
-    for (int j = 0; j < BWD_UNDER; ++j) {
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
+    for (long tb0 = t0; tb0 < t1 + K - 1; tb0 += UNDER) {
+    cur = next;
+    if (tb0 + UNDER < t1 + K - 1) fetch(tb0 + UNDER);
+#pragma unroll
+    for (int j = 0; j < UNDER; ++j) {
       const long t = tb0 + j;
       if (t >= t1 + K - 1) break;
       if (t < len) {
@@ -355,7 +386,7 @@ extern "C" int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int
   if (!dy || !x || !weight || !dx || (grad_initial_state && !initial_state)) return BKCORE_EINVAL;
   if (grad_params && (!workspace || workspace_bytes < bkcore_causal_conv_backward_workspace_bytes(B, L, C, K)))
     return BKCORE_EWORKSPACE;
-  const int v = 16 / elem_size(dtype);
+  constexpr int v = 4;  // channels a thread: eight would leave room for one wave a SIMD only
   const bool vec = C % v == 0 && x_batch % v == 0 && x_time % v == 0 && dy_batch % v == 0 && dy_time % v == 0 &&
                    aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(initial_state) &&
                    aligned16(grad_initial_state) && aligned16(grad_final_state);
@@ -369,7 +400,7 @@ extern "C" int bkcore_causal_conv_backward(const void *dy, int64_t dy_batch, int
 #define BK_CONV(K_, V_, AL_)                                                                                              \
   hipLaunchKernelGGL((bk_conv_backward_kernel<T, K_, V_, AL_>), dim3((unsigned)(B * nblk * cblk)), dim3(BWD_CH * BWD_SEGS), \
                      0, (hipStream_t)stream, a, (int)nblk, (int)cblk, (int)nvec)
-  BK_CONV_ANY(K, BK_CONV, (int)(16 / sizeof(T)), C >= v);
+  BK_CONV_ANY(K, BK_CONV, v, C >= v);
 #undef BK_CONV
   if (grad_params) bkcore_internal_sum_parts((const float *)workspace, B * nblk, (K + 1) * C, grad_params, stream);
   return launch_status();

@@ -209,3 +209,51 @@ def test_lm_of_kernels_trains_and_replays_from_a_graph(autocast):
     eager, captured = run(False), run(True)
     for a, b in zip(eager[1], captured[1]):
         torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-5)   # library products may take other kernels under capture
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once_do_not_meet():
+    """Every operator, forward and backward, on two streams with data of their own: the results of the calls alone."""
+    need_gpu()
+    import bkcore
+
+    def data(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, generator=g, device="cuda")
+        return dict(x=rn(2, 900, 96), w=rn(96), cw=rn(96, 4), A=-rn(96, 16).abs(), B=rn(2, 900, 16), C=rn(2, 900, 16),
+                    q=rn(2, 6, 900, 32), k=rn(2, 3, 900, 32), v=rn(2, 3, 900, 32))
+
+    def work(d):
+        t = {n: v.detach().requires_grad_() for n, v in d.items()}
+        y = bkcore.layer_norm(t["x"], t["w"])
+        u = bkcore.causal_conv(y, t["cw"], None, "silu")
+        s = bkcore.selective_scan(u, 0.1 * y, t["A"], t["B"], t["C"], delta_softplus=True)
+        o = bkcore.sliding_attention(t["q"], t["k"], t["v"], 40, 4)
+        grads = torch.autograd.grad([s.sum() + (o * o).sum()], list(t.values()))
+        return [s.detach(), o.detach(), *grads]
+    inputs = [data(1), data(2)]
+    alone = [work(d) for d in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    both = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                both[i] = work(inputs[i])
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_changed_inputs_are_noticed_by_the_backward():
+    need_gpu()
+    import bkcore
+    x = torch.randn(4, 32, device="cuda", requires_grad=True)
+    h = x * 1.0
+    y = bkcore.layer_norm(h)
+    h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
