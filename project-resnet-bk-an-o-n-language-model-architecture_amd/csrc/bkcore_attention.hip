@@ -20,7 +20,7 @@ int check(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t L, int64_t D, int
   if (!elem_size(dtype) || B < 0 || H < 1 || Hk < 1 || H % Hk || L < 0 || D < 1 || D > BKCORE_ATTENTION_MAX_HEAD_DIM)
     return BKCORE_EINVAL;
   if (window < 1 || sinks < 0 || sinks > BKCORE_ATTENTION_MAX_SINKS || scale != scale) return BKCORE_EINVAL;
-  if (B > (1 << 24) || H > (1 << 16) || L > (1 << 30)) return BKCORE_EINVAL;
+  if (B > (1 << 14) || H > (1 << 14) || L > (1 << 30)) return BKCORE_EINVAL;
   return BKCORE_OK;
 }
 

@@ -181,6 +181,13 @@ __device__ __forceinline__ long work_item(long total) {
   const long per = (total + 7) / 8, w = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
   return (long)(blockIdx.x >> 3) < per && w < total ? w : -1;
 }
+// The (batch, key head) of a run's g-th group: every eighth one after the other, so that sequences of unequal lengths (which
+// lie batch by batch) spread over the dies.
+__device__ __forceinline__ int work_group(int g, int groups) {
+  const int q = groups / 8, more = groups % 8, split = more * (q + 1);
+  if (g < split) return g % (q + 1) * 8 + g / (q + 1);
+  return (g - split) % q * 8 + more + (g - split) / q;
+}
 inline unsigned work_grid(long total) { return (unsigned)((total + 7) / 8 * 8); }
 
 template <typename T>
@@ -243,7 +250,7 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
   w /= G;
   const int qt = (int)(w % nq);
   w /= nq;
-  const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), h = hk * G + g_;
+  const int group = work_group((int)w, a.B * a.Hk), hk = group % a.Hk, b = group / a.Hk, h = hk * G + g_;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int len = row_length(a.lengths, b, a.L);
   const int q0 = qt * BM, q1 = min(q0 + BM, len) - 1;
@@ -421,7 +428,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
   w /= G;
   const int qt = (int)(w % nq);
   w /= nq;
-  const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), h = hk * G + g_;
+  const int group = work_group((int)w, a.B * a.Hk), hk = group % a.Hk, b = group / a.Hk, h = hk * G + g_;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int len = row_length(a.lengths, b, a.L);
   const int q0 = qt * BM, q1 = min(q0 + BM, len) - 1;
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
   w /= nk;
   const int split = (int)(w % ns);
   w /= ns;
-  const int hk = (int)(w % a.Hk), b = (int)(w / a.Hk), G = a.H / a.Hk;
+  const int group = work_group((int)w, a.B * a.Hk), hk = group % a.Hk, b = group / a.Hk, G = a.H / a.Hk;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
   const int len = row_length(a.lengths, b, a.L);
   const int key0 = SINK ? tile * WK : tile * BK + wave * WK;  // the wave's first key

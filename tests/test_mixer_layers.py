@@ -195,6 +195,8 @@ def test_lm_of_kernels_trains_and_replays_from_a_graph(autocast):
                 assert p.grad is not None and torch.isfinite(p.grad).all(), n
         if capture:
             opt.zero_grad(set_to_none=True)
+            for blk in m.blocks:
+                blk.bk_layer.last_g_ii = None      # it holds the warm-up's autograd graph, whose leaves the capture shares
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 loss = step()
