@@ -235,7 +235,13 @@ __device__ __forceinline__ int tile_view(int q0, int q1, int j0, int j1, int W, 
   if (j0 > q1 || (q0 - j1 >= W && j0 >= S)) return 0;
   return j1 <= q0 && (q1 - j0 < W || j1 < S) ? 2 : 1;
 }
-__device__ __forceinline__ bool sees(int i, int j, int W, int S) { return (j <= i) & ((i - j < W) | (j < S)); }
+// One unsigned comparison holds both ends of the window (a later key gives a huge distance); the sinks only where the tile
+// has some.
+template <bool SINKS>
+__device__ __forceinline__ bool sees(int i, int j, int W, int S) {
+  const unsigned gap = (unsigned)(i - j);
+  return SINKS ? (gap < (unsigned)W) | ((j < S) & (j <= i)) : gap < (unsigned)W;
+}
 
 // ---- forward: 4 waves x 16 QB queries; keys and values through LDS, the next tile on its way in registers.
 template <typename T, int DP, bool VEC, int QB>
@@ -319,11 +325,19 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[k][i][r] *= sc;
       if (view == 1) {
+        if (j0 < a.S) {
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+          for (int k = 0; k < NK; ++k)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[k][i][r] = sees(qi, j0 + 16 * k + 4 * g + r, a.W, a.S) ? s[k][i][r] : -INF;
+            for (int r = 0; r < 4; ++r)
+              s[k][i][r] = sees<true>(qi, j0 + 16 * k + 4 * g + r, a.W, a.S) ? s[k][i][r] : -INF;
+        } else {
+#pragma unroll
+          for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[k][i][r] = sees<false>(qi, j0 + 16 * k + 4 * g + r, a.W, a.S) ? s[k][i][r] : -INF;
+        }
       }
 #pragma unroll
       for (int k = 0; k < NK; ++k)
@@ -506,9 +520,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[i][r] = fmaf(s[i][r], sc, -lse[i]);
           if (view == 1) {
+            const int j = j0 + 16 * (k + kk) + 4 * g;
+            if (j0 < a.S) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              s[i][r] = sees(qi, j0 + 16 * (k + kk) + 4 * g + r, a.W, a.S) ? s[i][r] : -INF;
+              for (int r = 0; r < 4; ++r) s[i][r] = sees<true>(qi, j + r, a.W, a.S) ? s[i][r] : -INF;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[i][r] = sees<false>(qi, j + r, a.W, a.S) ? s[i][r] : -INF;
+            }
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -678,10 +697,11 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
         for (int r = 0; r < 4; ++r) s[y][r] = fmaf(s[y][r], sc, -ls[r]);
       if (view == 1) {
 #pragma unroll
-        for (int y = 0; y < KB; ++y)
+        for (int y = 0; y < KB; ++y) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            s[y][r] = sees(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? s[y][r] : -INF;
+            s[y][r] = sees<true>(i0 + 16 * x + 4 * g + r, key0 + 16 * y + m, a.W, a.S) ? s[y][r] : -INF;
+        }
       }
 #pragma unroll
       for (int y = 0; y < KB; ++y)
