@@ -7,6 +7,8 @@
 // row up to 2048 elements (no barrier at all), a workgroup beyond.  The backward's threads keep their columns over all
 // the rows they visit, so the sums over rows stay in registers until one partial row a workgroup is written; a second
 // launch adds the partial rows in a fixed order.  Statistics and sums are float32.
+// Measured at 16384 x 2048 bf16: forward 23 us (5.8 TB/s), backward 40 + 4 us (4.6 TB/s; without the prefetch of the next
+// row 64); 4099 x 1537 f16, rows at odd addresses: 8.4 us (14.7 with one element an access).
 #include "bkcore_types.h"
 
 namespace {

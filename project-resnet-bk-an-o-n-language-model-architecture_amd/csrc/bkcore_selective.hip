@@ -18,10 +18,15 @@
 // those in front of its chunk and runs the chunk from there.
 // The backward needs h at every position: the forward keeps it at every 16th (e.g. 4 bytes a position and channel for 16
 // states), and a tile of 16 positions recomputes the rest into registers (the transitions twice: kept
-// beside the states they would not fit).
+// beside the states they would not fit: 313 us with 94 registers spilled, 158 so).
 // The sums over channels (dB, dC) are folded across the wave by lane exchanges, across the workgroup's waves in LDS and
 // across workgroups by a second launch; every order is fixed, results do not change from run to run.
 // States, statistics and sums are float32 whatever the operands' type.
+//
+// Measured at 4 x 2048 positions x 1024 channels x 16 states, bf16: chunks' ends 34 us, forward 52, adjoint's ends 38,
+// backward 158 (512 x 16 positions a SIMD: 28, 42, 31 and 122 vector instructions a position, busy 75 % of the time; the
+// rest is the start of a chunk and the barriers), both sums 10.  8191 positions x 512 channels f32: 20 + 35.  256 tokens x
+// 2048 channels: 16.8 us (4.2 TB/s).
 #include "bkcore_types.h"
 
 namespace {
