@@ -116,7 +116,7 @@ extern "C" int bkcore_sliding_attention_backward(
   if (rc) return rc;
   if (B == 0 || L == 0) return BKCORE_OK;
   if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return BKCORE_EINVAL;
-  if (B * H * L > 2147483000LL * 16 || B * H * ((L + 63) / 64) > 2147483000LL) return BKCORE_EINVAL;
+  if (B * H * ((L + 63) / 64) > 2147483000LL) return BKCORE_EINVAL;
   if (!workspace || workspace_bytes < bkcore_sliding_attention_backward_workspace_bytes(B, H, Hk, L, D, window, sinks))
     return BKCORE_EWORKSPACE;
   AttnArgs a{};

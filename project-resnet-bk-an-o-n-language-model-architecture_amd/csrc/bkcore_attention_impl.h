@@ -14,10 +14,10 @@
 // What bounds it: in the prompts and in training the vector unit (one exponential and about ten instructions a score), the
 // matrix unit and LDS take a like share each of a tile's time, and two waves a SIMD hide only part of one behind another.
 // Measured at 2 x 16 heads x 8192 x 128 bf16 over 4 key heads, window 1024, 4 sinks: forward 246 us (129 GFLOP: 0.53 PFLOP/s),
-// delta 31, dk and dv 424 + 44 + 5 (the sinks' part and its join apart), dq 325; both form the scores again, so the backward
-// does nine products of this size for the five it needs (two of the nine are the second halves of the score gradients);
-// 4 x 8 heads x 3001 ragged x 64 f16, window 500: 31.  The single-token step is bound by the cache's
-// bytes: 64 sequences x 32 heads over 8 x 4100 slots x 128 bf16 in 171 + 5 us = 5.7 TB/s.
+// dq with delta 345 (delta in a launch of its own: 325 + 31), dk and dv 424 + 44 + 5 (the sinks' part and its join apart);
+// both form the scores again, so the backward does nine products of this size for the five it needs (two of the nine are
+// the second halves of the score gradients); 4 x 8 heads x 3001 ragged x 64 f16, window 500: 31.  The single-token step is
+// bound by the cache's bytes: 64 sequences x 32 heads over 8 x 4100 slots x 128 bf16 in 171 + 5 us = 5.7 TB/s.
 #include "bkcore_attention.h"
 
 namespace bk {
@@ -408,36 +408,9 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
   }
 }
 
-// ---- delta_i = do_i . o_i: a row's D elements over TPR = DP / 8 lanes.  A 16-bit output's rounding is added back (lo):
-// it would reach every score gradient of the row.
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(256) void bk_attn_delta_kernel(AttnArgs a) {
-  constexpr int TPR = DP / 8;
-  const long id = ((long)blockIdx.x * 256 + threadIdx.x) / TPR;
-  const int c = (threadIdx.x % TPR) * 8;
-  const long total = (long)a.B * a.L * a.H;
-  const long i = id < total ? id : total - 1;
-  const int h = (int)(i % a.H);
-  const long bt = i / a.H;
-  const int b = (int)(bt / a.L), t = (int)(bt % a.L);
-  const Frag<T> o = load8<T, VEC>((const T *)a.out + i * a.D, c, a.D);
-  const Frag<T> gr = load8<T, VEC>(head<T>(a.dout, b, h) + (long)t * a.dout.t, c, a.D);
-  Frag<T> lo;
-  if (a.lo) lo = load8<T, VEC>((const T *)a.lo + i * a.D, c, a.D);
-  float s = 0.0f;
-  if (t < row_length(a.lengths, b, a.L)) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < a.D) s = fmaf((float)o.v[k] + (a.lo ? (float)lo.v[k] : 0.0f), (float)gr.v[k], s);
-  }
-  s += dpp_mov<DPP_XOR1>(s);
-  s += dpp_mov<DPP_XOR2>(s);
-  if constexpr (TPR >= 8) s += dpp_mov<DPP_HALF_MIRROR>(s);
-  if constexpr (TPR >= 16) s += dpp_mov<DPP_MIRROR>(s);
-  if (id < total && c == 0) a.delta[((long)b * a.H + h) * a.L + t] = s;
-}
-
-// ---- dq: the forward's loop with two score products, dS^T in the lane, and K contracted over its rows.
+// ---- dq: the forward's loop with two score products, dS^T in the lane, and K contracted over its rows.  It runs first and
+// leaves delta_i = do_i . o_i for the keys' launch: a row's gradient is in its registers anyway.  A 16-bit output's rounding
+// is added back (lo): it would reach every score gradient of the row.
 template <typename T, int DP, bool VEC, int QB>
 __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_kernel(AttnArgs a) {
   constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32, WQ = 16 * QB, BM = 4 * WQ;
@@ -472,15 +445,31 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
         q[i][c] = load8<T, VEC>(qp + r * a.q.t, c * 32 + g * 8, a.D);
         go[i][c] = load8<T, VEC>(gp + r * a.dout.t, c * 32 + g * 8, a.D);
       }
-      const float l_ = a.lse[((long)b * a.H + h) * a.L + r], d_ = a.delta[((long)b * a.H + h) * a.L + r];
-      if (row < len) {
-        lse[i] = l_;
-        delta[i] = d_;
+      const T *orow = (const T *)a.out + (((long)b * a.L + r) * a.H + h) * a.D;
+      const T *lrow = (const T *)a.lo + (((long)b * a.L + r) * a.H + h) * a.D;
+      Frag<T> oo[NC], ol[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        oo[c] = load8<T, VEC>(orow, c * 32 + g * 8, a.D);
+        if (a.lo) ol[c] = load8<T, VEC>(lrow, c * 32 + g * 8, a.D);
       }
+      const float l_ = a.lse[((long)b * a.H + h) * a.L + r];
+      float dot = 0.0f;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         q[i][c] = zero_unless<T, VEC>(q[i][c], row < len, c * 32 + g * 8, a.D);
         go[i][c] = zero_unless<T, VEC>(go[i][c], row < len, c * 32 + g * 8, a.D);
+        oo[c] = zero_unless<T, VEC>(oo[c], row < len, c * 32 + g * 8, a.D);
+        if (a.lo) ol[c] = zero_unless<T, VEC>(ol[c], row < len, c * 32 + g * 8, a.D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          dot = fmaf((float)oo[c].v[e] + (a.lo ? (float)ol[c].v[e] : 0.0f), (float)go[i][c].v[e], dot);
+      }
+      dot = col_sum(dot);  // over the four lanes that share the row
+      if (row < len) {
+        lse[i] = l_;
+        delta[i] = dot;
+        if (g == 0) a.delta[((long)b * a.H + h) * a.L + row] = dot;
       }
     }
 #pragma unroll
@@ -984,8 +973,7 @@ void attn_forward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
 
 template <typename T>
 void attn_backward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
-  const long rows = (long)a.B * a.H * a.L, heads = (long)a.B * a.H, kheads = (long)a.B * a.Hk;
-  const unsigned grid_d = (unsigned)((rows * (dp / 8) + 255) / 256);
+  const long heads = (long)a.B * a.H, kheads = (long)a.B * a.Hk;
 #define BK_LAUNCH_Q(DP, VEC, QB)                                                                                      \
   hipLaunchKernelGGL((bk_attn_dq_kernel<T, DP, VEC, QB>), dim3(work_grid(heads * ((a.L + 64 * QB - 1) / (64 * QB)))), \
                      dim3(256), 0, s, a)
@@ -997,13 +985,12 @@ void attn_backward(const AttnArgs &a, int dp, bool vec, hipStream_t s) {
                      dim3(work_grid(kheads * ((a.S + 16 * KB - 1) / (16 * KB)) * a.nsplit)), dim3(256), 0, s, a)
 #define BK_LAUNCH(DP, VEC)                                                                        \
   do {                                                                                            \
-    hipLaunchKernelGGL((bk_attn_delta_kernel<T, DP, VEC>), dim3(grid_d), dim3(256), 0, s, a);     \
+    if (a.wide_q) BK_LAUNCH_Q(DP, VEC, 2);                                                        \
+    else BK_LAUNCH_Q(DP, VEC, 1);                                                                 \
     if (a.wide_k) BK_LAUNCH_K(DP, VEC, 2);                                                        \
     else BK_LAUNCH_K(DP, VEC, 1);                                                                 \
     if (a.nsplit && a.S > 16) BK_LAUNCH_S(DP, VEC, 2);                                            \
     else if (a.nsplit) BK_LAUNCH_S(DP, VEC, 1);                                                   \
-    if (a.wide_q) BK_LAUNCH_Q(DP, VEC, 2);                                                        \
-    else BK_LAUNCH_Q(DP, VEC, 1);                                                                 \
   } while (0)
   BK_ATTN_DP(BK_LAUNCH);
 #undef BK_LAUNCH

@@ -6,8 +6,7 @@ from test_kernel_resources import _find, kernels  # noqa: F401
 
 def test_hot_loops_do_not_spill(kernels):  # noqa: F811
     names = ["bk_scan_kernel", "bk_scan_adjoint_agg_kernel", "bk_scan_backward_kernel", "bk_scan_step_kernel", "bk_conv_kernel",
-             "bk_conv_step_kernel", "bk_layer_norm_kernel", "bk_attn_kernelIDF16", "bk_attn_step_kernel",
-             "bk_attn_delta_kernel"]
+             "bk_conv_step_kernel", "bk_layer_norm_kernel", "bk_attn_kernelIDF16", "bk_attn_step_kernel"]
     for name in names:
         for k in _find(kernels, name):
             assert kernels[k]["private_segment_fixed_size"] == 0, (k, kernels[k])
