@@ -71,9 +71,15 @@ def _cache(what: str, q: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, v
             raise ValueError(f"bkcore: {what}: {name} is (B, Hk, slots, D), got {tuple(c.shape)}")
         if c.shape[3] > 1 and c.stride(3) != 1:
             raise ValueError(f"bkcore: {what}: the last dimension of {name} must be contiguous")
-        if c.shape[2] > 1 and c.stride(2) < c.shape[3]:
-            raise ValueError(f"bkcore: {what}: the slots of {name} overlap")
+        if not c.is_contiguous():
+            reach = 1
+            for stride, size in sorted((c.stride(i), c.shape[i]) for i in range(4) if c.shape[i] > 1):
+                if stride < reach:
+                    raise ValueError(f"bkcore: {what}: slots of {name} overlap")
+                reach += stride * (size - 1)
         ops.need_state(what, name, c, q, tuple(c.shape), q.dtype)
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
+        raise ValueError(f"bkcore: {what}: k_cache and v_cache are the same memory")
     if k_cache.shape[2] <= sinks:
         raise ValueError(f"bkcore: {what}: {k_cache.shape[2]} slots leave none behind {sinks} sinks")
     return k_cache.shape[2]
@@ -98,7 +104,7 @@ def sliding_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
                            positions: torch.Tensor, window: int, sinks: int = 0,
                            scale: float | None = None) -> torch.Tensor:
     """``sliding_attention`` for one token of each sequence: q (B, H, D), k and v (B, Hk, D) of the token at ``positions``
-    (B,), which are written into the rolling caches (see ``sliding_cache_fill``; at least ``window + sinks`` slots) in place.
+    (B,), below 2**31, which are written into the rolling caches (see ``sliding_cache_fill``; at least ``window + sinks`` slots) in place.
     A negative position leaves its sequence alone: output zero, cache as it was.  No gradient."""
     what = "sliding_attention_step"
     _heads(what, q, k, v, 3)

@@ -796,7 +796,7 @@ __global__ __launch_bounds__(256) void bk_attn_step_kernel(StepArgs a) {
   const T *kn = head<T>(a.k, b, hk), *vn = head<T>(a.v, b, hk);
   const int ring = a.cap - a.S;
   const int first = max(a.S, pos - a.W + 1);                     // first position of the window behind the sinks
-  const int nsink = pos < 0 ? 0 : min(a.S, pos + 1), n = pos < 0 ? 0 : nsink + max(0, pos - first + 1);
+  const int nsink = pos < 0 ? 0 : min(a.S - 1, pos) + 1, n = pos < 0 ? 0 : nsink + max(0, pos - first + 1);
   auto slot = [&](int t) {  // of the t-th visible position
     return t < nsink ? t : a.S + (first - a.S + t - nsink) % ring;
   };

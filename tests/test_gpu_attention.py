@@ -292,3 +292,38 @@ def test_empty_and_refusals():
         bkcore.sliding_cache_fill(k, v, kc[:, :, :4], kc[:, :, :4], None, 4)
     with pytest.raises(TypeError):
         bkcore.sliding_cache_fill(k, v, kc.float(), kc.float())
+
+
+def test_caches_that_share_memory_are_refused():
+    import bkcore
+    q, k, v, _ = (t.cuda() for t in inputs(2, 4, 2, 8, 16, BF16))
+    qs, ks, vs = q[:, :, 0], k[:, :, 0], v[:, :, 0]
+    kc, vc = (torch.zeros(2, 2, 12, 16, dtype=BF16, device="cuda") for _ in range(2))
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    shared = (kc[:1].expand(2, -1, -1, -1), kc[:, :1].expand(-1, 2, -1, -1),
+              kc.view(-1).as_strided((2, 2, 12, 16), (200, 192, 16, 1)))
+    for a, b in [(kc, kc)] + [(c, vc) for c in shared] + [(vc, c) for c in shared]:
+        with pytest.raises(ValueError):
+            bkcore.sliding_attention_step(qs, ks, vs, a, b, pos, 4, 2)
+        with pytest.raises(ValueError):
+            bkcore.sliding_cache_fill(k, v, a, b)
+    both = torch.zeros(2, 12, 2, 2, 16, dtype=BF16, device="cuda")       # keys and values side by side in a slot
+    a, b = both.permute(3, 0, 2, 1, 4)
+    got = bkcore.sliding_attention_step(qs, ks, vs, a, b, pos, 4, 2)
+    assert torch.equal(got, vs.repeat_interleave(2, 1)) and torch.equal(a[:, :, 0], ks) and torch.equal(b[:, :, 0], vs)
+
+
+@pytest.mark.parametrize("position", [2 ** 31 - 2, 2 ** 31 - 1])
+def test_step_at_the_last_positions(position):
+    """Two slots behind two sinks: the token itself and the one in front of it, next to the sinks."""
+    import bkcore
+    q, k, v, _ = (t.cuda() for t in inputs(1, 2, 2, 4, 16, torch.float32))
+    kc, vc = (torch.empty(1, 2, 4, 16, device="cuda") for _ in range(2))
+    at = [0, 1, 2 + (position - 3) % 2, 2 + (position - 2) % 2]
+    kc[:, :, at], vc[:, :, at] = k, v
+    kc[:, :, at[3]], vc[:, :, at[3]] = float("nan"), float("nan")
+    pos = torch.tensor([position], dtype=torch.int64, device="cuda")
+    got = bkcore.sliding_attention_step(q[:, :, 3], k[:, :, 3], v[:, :, 3], kc, vc, pos, 2, 2)
+    want = attention(*d64(q, k, v), 4, 0, 16 ** -0.5, half_step(torch.float32))
+    assert_within(got, want["o"][:, :, 3], want["eo"][:, :, 3])
+    assert torch.equal(kc[:, :, at], k) and torch.equal(vc[:, :, at], v)
