@@ -6,8 +6,8 @@ token + position embedding, pre-norm residual blocks whose mixing path is the BK
 network, final LayerNorm, vocabulary head).  ``hybrid=True`` selects what configs/phase7_small.yaml:11 selects in the
 reference (``use_hybrid_attention``): the block's mixing path is gated by the resolvent diagonal
 (``bkcore.layers.BKHybridLayer``: the reference's gate, resnet_bk.py:172-185 and hybrid_attention.py:117-143, around
-stand-in local and global paths, or the library's sliding-window attention and
-selective mixer: ``local``, ``sinks``, ``global_path``), the features go unused and the operator's backward sees a cotangent on G_ii alone.
+stand-in local and global paths, or the library's sliding-window attention and selective mixer: ``local``, ``sinks``,
+``global_path``), the features go unused and the operator's backward sees a cotangent on G_ii alone.
 MoE routing and the HTT embedding are not part of it.  What it exercises is the operator inside a real backward pass and, with more than one
 process, the data-parallel gradient all-reduce around it.
 """
