@@ -410,7 +410,9 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
 
 // ---- dq: the forward's loop with two score products, dS^T in the lane, and K contracted over its rows.  It runs first and
 // leaves delta_i = do_i . o_i for the keys' launch: a row's gradient is in its registers anyway.  A 16-bit output's rounding
-// is added back (lo): it would reach every score gradient of the row.
+// is added back (lo): it would reach every score gradient of the row.  delta is the diagonal of the same matrix product, in
+// the same order, that gives do_i . v_j: a row that sees one key has o_i = v_j, and its score gradient do_i . v_j - delta_i
+// is zero to the last bit, as it is by the formula (a sum in another order leaves 1e-7 of its terms there).
 template <typename T, int DP, bool VEC, int QB>
 __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_kernel(AttnArgs a) {
   constexpr int BN = key_tile<T>(), LD = DP + pad<T>(), NK = BN / 16, ND = DP / 16, NC = DP / 32, WQ = 16 * QB, BM = 4 * WQ;
@@ -454,18 +456,22 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
         if (a.lo) ol[c] = load8<T, VEC>(lrow, c * 32 + g * 8, a.D);
       }
       const float l_ = a.lse[((long)b * a.H + h) * a.L + r];
-      float dot = 0.0f;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         q[i][c] = zero_unless<T, VEC>(q[i][c], row < len, c * 32 + g * 8, a.D);
         go[i][c] = zero_unless<T, VEC>(go[i][c], row < len, c * 32 + g * 8, a.D);
         oo[c] = zero_unless<T, VEC>(oo[c], row < len, c * 32 + g * 8, a.D);
         if (a.lo) ol[c] = zero_unless<T, VEC>(ol[c], row < len, c * 32 + g * 8, a.D);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          dot = fmaf((float)oo[c].v[e] + (a.lo ? (float)ol[c].v[e] : 0.0f), (float)go[i][c].v[e], dot);
       }
-      dot = col_sum(dot);  // over the four lanes that share the row
+      f32x4 od = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) mma(oo[c], go[i][c], od);
+      if (a.lo) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) mma(ol[c], go[i][c], od);
+      }
+      const float mine = (m & 2) ? ((m & 1) ? od[3] : od[2]) : ((m & 1) ? od[1] : od[0]);
+      const float dot = col_sum(g == (m >> 2) ? mine : 0.0f);  // to the four lanes that share the row
       if (row < len) {
         lse[i] = l_;
         delta[i] = dot;
