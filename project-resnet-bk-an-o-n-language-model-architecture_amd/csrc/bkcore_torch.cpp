@@ -53,6 +53,11 @@ Tensor floats(const Tensor &like, at::IntArrayRef shape) { return at::empty(shap
 Tensor bytes(const Tensor &like, size_t n) {
   return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
 }
+// A caller's buffer was written through its pointer: functions that saved it for their backward have to notice, as they do
+// after the tensor library's own in-place operations.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 using Optional = std::optional<Tensor>;
 // An absent operand has no place among a node's edges, so a later operand's edge is counted over those that are there.
 Tensor opt(const std::optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
@@ -179,6 +184,7 @@ Tensor causal_conv_step(const Tensor &x_, const Tensor &state, const Tensor &wei
   check(bkcore_causal_conv_step(x.data_ptr(), x.stride(0), dtype_of(x), state.data_ptr(), w.data_ptr(), ptr(b), dtype_of(w), B,
                                 C, K, (int)silu, y.data_ptr(), handle(stream)),
         "bkcore_causal_conv_step");
+  written(state);
   return y;
 }
 
@@ -277,6 +283,7 @@ Tensor selective_scan_step(const Tensor &x_, const Tensor &state, const Tensor &
                                    Bm.data_ptr(), Bm.stride(0), Cm.data_ptr(), Cm.stride(0), fptr(D), ptr(z), str(z, 0),
                                    fptr(bias), (int)softplus, dtype_of(x), B, C, N, y.data_ptr(), handle(stream)),
         "bkcore_selective_scan_step");
+  written(state);
   return y;
 }
 
@@ -346,6 +353,8 @@ Tensor sliding_attention_step(const Tensor &q_, const Tensor &k_, const Tensor &
                                       iptr(positions), dtype_of(q), B, H, Hk, cap, D, window, sinks, (float)scale,
                                       o.data_ptr(), ptr(ws), n, handle(stream)),
         "bkcore_sliding_attention_step");
+  written(kc);
+  written(vc);
   return o;
 }
 
@@ -357,6 +366,8 @@ void sliding_cache_fill(const Tensor &k_, const Tensor &v_, const Tensor &kc, co
                                   vc.data_ptr(), vc.stride(0), vc.stride(1), vc.stride(2), iptr(lengths), dtype_of(k),
                                   k.size(0), k.size(1), k.size(2), kc.size(2), k.size(3), sinks, handle(stream)),
         "bkcore_sliding_cache_fill");
+  written(kc);
+  written(vc);
 }
 
 }  // namespace
