@@ -58,6 +58,12 @@ Tensor bytes(const Tensor &like, size_t n) {
 void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// Calls without a derivative refuse forward-mode tangents, which would be lost without a word.
+void no_tangent(const char *what, std::initializer_list<Tensor> operands) {
+  for (const Tensor &t : operands)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "bkcore: ", what, " has no derivative, and an operand carries a "
+                "forward-mode tangent");
+}
 using Optional = std::optional<Tensor>;
 // An absent operand has no place among a node's edges, so a later operand's edge is counted over those that are there.
 Tensor opt(const std::optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
@@ -178,6 +184,7 @@ variable_list causal_conv(const Tensor &x, const Tensor &w, const Optional &b, c
 
 Tensor causal_conv_step(const Tensor &x_, const Tensor &state, const Tensor &weight, const Optional &bias,
                         int64_t silu, int64_t stream) {
+  no_tangent("causal_conv_step", {x_, state, weight, opt(bias)});
   const Tensor x = inner(x_), w = dense(weight), b = dense(opt(bias));
   const int64_t B = x.size(0), C = x.size(1), K = w.size(1);
   Tensor y = at::empty({B, C}, x.options());
@@ -273,6 +280,7 @@ variable_list selective_scan(const Tensor &x, const Tensor &delta, const Tensor 
 Tensor selective_scan_step(const Tensor &x_, const Tensor &state, const Tensor &delta_, const Tensor &A_, const Tensor &B_,
                            const Tensor &C_, const Optional &D_, const Optional &z_,
                            const Optional &bias_, int64_t softplus, int64_t stream) {
+  no_tangent("selective_scan_step", {x_, state, delta_, A_, B_, C_, opt(D_), opt(z_), opt(bias_)});
   const Tensor x = inner(x_), delta = inner(delta_), Bm = inner(B_), Cm = inner(C_), z = inner(opt(z_));
   const Tensor D = dense(opt(D_)), bias = dense(opt(bias_));
   Tensor A = dense(A_);
@@ -342,6 +350,7 @@ Tensor sliding_attention(const Tensor &q, const Tensor &k, const Tensor &v, cons
 
 Tensor sliding_attention_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &kc, const Tensor &vc,
                               const Tensor &positions_, int64_t window, int64_t sinks, double scale, int64_t stream) {
+  no_tangent("sliding_attention_step", {q_, k_, v_, kc, vc});
   const Tensor q = inner(q_), k = inner(k_), v = inner(v_), positions = positions_.contiguous();
   const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hk = k.size(1), cap = kc.size(2);
   Tensor o = at::empty({B, H, D}, q.options());
@@ -360,6 +369,7 @@ Tensor sliding_attention_step(const Tensor &q_, const Tensor &k_, const Tensor &
 
 void sliding_cache_fill(const Tensor &k_, const Tensor &v_, const Tensor &kc, const Tensor &vc,
                         const Optional &lengths_, int64_t sinks, int64_t stream) {
+  no_tangent("sliding_cache_fill", {k_, v_, kc, vc});
   const Tensor k = inner(k_), v = inner(v_), lengths = opt(lengths_);
   check(bkcore_sliding_cache_fill(k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0),
                                   v.stride(1), v.stride(2), kc.data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2),
