@@ -50,7 +50,8 @@ def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     share a key / value head), D <= 128, at most 64 sinks; ``scale`` defaults to D ** -0.5.  Heads and positions may have any
     strides (slices of one projection).  The result (B, H, L, D) has its heads inside a position in memory.
 
-    Scores, softmax and sums are float32; probabilities enter the product with v in the operands' type.  A non-finite key
+    Scores, softmax and sums are float32; probabilities and score gradients enter their products as two values of the
+    operands' type, so results are as near as their own rounding.  A non-finite key
     or value inside a sequence may reach any row that works on the same tile of keys, not only those that see it."""
     what = "sliding_attention"
     _heads(what, q, k, v, 4)

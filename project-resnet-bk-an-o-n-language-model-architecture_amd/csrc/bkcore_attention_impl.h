@@ -140,27 +140,33 @@ __device__ __forceinline__ Frag<T> across(const T *lds, int row0, int col0, int 
   return f;
 }
 
-// A score's gradient as two values of the operands' type, what rounding takes from the first in the second: the gradients
-// of a row sum to zero, so their products with K and Q cancel, and one rounding of half a step each would be half as much
-// again as the rounding of the result (0.0026 of dq's size against 0.0017 in bfloat16).
+// Four neighbouring values of a lane as elements i0 .. i0 + 3 of two operands, what rounding takes from the first in the
+// second.  Score gradients: those of a row sum to zero, so their products with K and Q cancel, and one rounding of half a
+// step each would be half as much again as the rounding of the result (0.0026 of dq's size against 0.0017 in bfloat16).
+// Probabilities: rounded once they would leave the output and dv 1.3 times as far from the formula as the rounding of the
+// result does (0.0022 against 0.0017).  The second products cost 10 % of a training pass and 20 % of a prompt.
+// (float16 goes through the packed conversion, which cuts instead of rounding: the second value takes that up too.)
 template <typename T>
-__device__ __forceinline__ void put_split(float x, int i, Frag<T> &hi, Frag<T> &lo) {
-  const T h = (T)x;
-  hi.v[i] = h;
-  lo.v[i] = (T)(x - (float)h);
-}
-
-// Two 16-row blocks of a score column as one operand, rounded to the operands' type: probabilities enter the product with
-// V in the precision of the values they multiply (nothing cancels there), their sum stays float32.
-template <typename T>
-__device__ __forceinline__ Frag<T> to_frag(const f32x4 &lo, const f32x4 &hi) {
-  Frag<T> f;
+__device__ __forceinline__ void put_split(const f32x4 &x, int i0, Frag<T> &hi, Frag<T> &lo) {
+  if constexpr (__is_same(T, f16_t)) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f.v[i] = (T)lo[i];
-    f.v[4 + i] = (T)hi[i];
+    for (int i = 0; i < 4; i += 2) {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
+      const auto l = __builtin_amdgcn_cvt_pkrtz(x[i] - (float)h[0], x[i + 1] - (float)h[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        hi.v[i0 + i + k] = (T)h[k];
+        lo.v[i0 + i + k] = (T)l[k];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T h = (T)x[i];
+      hi.v[i0 + i] = h;
+      lo.v[i0 + i] = (T)(x[i] - (float)h);
+    }
   }
-  return f;
 }
 
 // Maximum / sum over the four lanes that hold one column (l, l + 16, l + 32, l + 48), in each of them.
@@ -370,14 +376,21 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < NK; k += 2) {
-      Frag<T> p[QB];
+      Frag<T> p[QB], pl[QB];
 #pragma unroll
-      for (int i = 0; i < QB; ++i) p[i] = to_frag<T>(s[k][i], s[k + 1][i]);
+      for (int i = 0; i < QB; ++i) {
+        put_split(s[k][i], 0, p[i], pl[i]);
+        put_split(s[k + 1][i], 4, p[i], pl[i]);
+      }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const Frag<T> vf = across<T, DP>(sV, 16 * k, 16 * d, lane);
 #pragma unroll
         for (int i = 0; i < QB; ++i) mma(vf, p[i], o[d][i]);
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int i = 0; i < QB; ++i) mma(vf, pl[i], o[d][i]);
+        }
       }
     }
   }
@@ -533,8 +546,8 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
             }
           }
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            put_split(exp2_fast(s[i][r]) * (dp[i][r] - delta[i]), 4 * kk + r, ds[i], dl[i]);
+          for (int r = 0; r < 4; ++r) dp[i][r] = exp2_fast(s[i][r]) * (dp[i][r] - delta[i]);
+          put_split(dp[i], 4 * kk, ds[i], dl[i]);
         }
       }
 #pragma unroll
@@ -672,7 +685,7 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
     const int i0 = (int)qi + sub;
     const int view = i0 < len && key0 < len ? tile_view(i0, i0 + BQ - 1, key0, key0 + WK - 1, a.W, a.S) : 0;
     if (!view) continue;
-    Frag<T> pf[KB], df[KB], dl[KB];
+    Frag<T> pf[KB], pl[KB], df[KB], dl[KB];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       f32x4 s[KB], dp[KB];  // of the key blocks: a lane holds four queries of one key
@@ -707,13 +720,15 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
         }
       }
 #pragma unroll
-      for (int y = 0; y < KB; ++y)
+      for (int y = 0; y < KB; ++y) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = exp2_fast(s[y][r]);
-          pf[y].v[4 * x + r] = (T)p;
-          put_split(p * (dp[y][r] - de[r]), 4 * x + r, df[y], dl[y]);
+          s[y][r] = exp2_fast(s[y][r]);
+          dp[y][r] = s[y][r] * (dp[y][r] - de[r]);
         }
+        put_split(s[y], 4 * x, pf[y], pl[y]);
+        put_split(dp[y], 4 * x, df[y], dl[y]);
+      }
       if constexpr (VLDS) __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -726,7 +741,10 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
       }
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int y = 0; y < KB; ++y) mma(qt, dl[y], dk[d][y]);
+        for (int y = 0; y < KB; ++y) {
+          mma(qt, dl[y], dk[d][y]);
+          mma(gt, pl[y], dv[d][y]);
+        }
       }
       if constexpr (VLDS) {
         if (d & 1) __builtin_amdgcn_sched_barrier(0);
@@ -887,12 +905,16 @@ __global__ __launch_bounds__(256) void bk_attn_step_kernel(StepArgs a) {
         part += s[k][r];
       }
     sum = fmaf(sum, alpha, part);
-    const Frag<T> p = to_frag<T>(s[0], s[1]);
+    Frag<T> p, pl;
+    put_split(s[0], 0, p, pl);
+    put_split(s[1], 4, p, pl);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[d][r] *= alpha;
-      mma(across<T, DP>(sV, 0, 16 * d, lane), p, o[d]);
+      const Frag<T> vf = across<T, DP>(sV, 0, 16 * d, lane);
+      mma(vf, p, o[d]);
+      if constexpr (sizeof(T) == 2) mma(vf, pl, o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }

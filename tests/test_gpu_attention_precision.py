@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from mixer_reference import assert_within
+from attention_bounds import NEAR, rounding_ratio
+from mixer_reference import assert_within, attention, d64
 from test_gpu_attention import BF16, F16, F32, inputs
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,30 @@ def test_first_rows_have_no_score_gradient(dtype):
     # exponential 2^-23
     g = do[:, :, 0].cpu().double().view(2, 2, 2, 64)
     assert_within(dv[:, :, 0], g.sum(2), 2.0 ** -21 * g.abs().sum(2))
+
+
+# lengths with and without a part of the sinks behind the first keys, shared heads, a batch that takes 128 rows a workgroup
+@pytest.mark.parametrize("B,H,Hk,L,D,window,sinks", [(1, 2, 1, 257, 32, 31, 33), (2, 2, 2, 400, 128, 8, 64), (1, 4, 4, 150, 64, 40, 3),
+                                                     (1, 2, 1, 900, 64, 300, 4), (6, 16, 16, 300, 128, 150, 4), (1, 3, 3, 300, 73, 60, 2)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_results_are_as_near_as_their_rounding(B, H, Hk, L, D, window, sinks, dtype):
+    q, k, v, do = inputs(B, H, Hk, L, D, dtype, seed=L)
+    got = train(*(t.cuda() for t in (q, k, v, do)), window, sinks)
+    r = attention(*d64(q, k, v), window, sinks, D ** -0.5, 0.0, None, d64(do))
+    for t, n in zip(got, ("o", "dq", "dk", "dv")):
+        assert rounding_ratio(t, r[n]) <= NEAR, n
+
+
+@pytest.mark.parametrize("B,H,Hk,D,window,sinks", [(4, 8, 2, 64, 400, 4), (16, 16, 16, 128, 30, 2), (1, 5, 1, 73, 800, 0)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_single_tokens_are_as_near_as_their_rounding(B, H, Hk, D, window, sinks, dtype):
+    """At the last position that fills the cache every slot is visible, in any order."""
+    import bkcore
+    slots = window + sinks
+    q, k, v, _ = inputs(B, H, Hk, slots, D, dtype, seed=D)
+    kc, vc = k.cuda(), v.cuda()
+    pos = torch.full((B,), slots - 1, dtype=torch.int32, device="cuda")
+    got = bkcore.sliding_attention_step(q[:, :, -1].cuda(), k[:, :, -1].cuda(), v[:, :, -1].cuda(), kc, vc, pos, window, sinks)
+    K, V = (t.double().repeat_interleave(H // Hk, 1) for t in (k, v))
+    p = torch.softmax((K @ q[:, :, -1, :, None].double())[..., 0] * D ** -0.5, -1)
+    assert rounding_ratio(got, (p[..., None] * V).sum(2)) <= NEAR
