@@ -433,7 +433,8 @@ int bkcore_selective_scan_step(const void *x, int64_t x_batch, float *state, con
  * heads share one).  Takes the place of the windowed local path (src/models/phase7/hybrid_attention.py:93-103), whose
  * windows are blocks.  q (B, H, L, D), k, v (B, Hk, L, D) by strides, D <= 128; out (B, L, H, D) contiguous; lse: NULL, or
  * (B, H, L) floats for the backward (base-2 logarithm of the row's sum; +inf for a row that sees nothing); out_lo: NULL, or
- * what rounding took from out (out's layout and type), which the backward adds back where the output enters it. */
+ * what rounding took from out (out's layout and type; in BKCORE_F16 times 2^11), which the backward adds back where the
+ * output enters it. */
 #define BKCORE_ATTENTION_MAX_HEAD_DIM 128
 #define BKCORE_ATTENTION_MAX_SINKS 64
 int bkcore_sliding_attention(const void *q, int64_t q_batch, int64_t q_head, int64_t q_time, const void *k,

@@ -43,6 +43,22 @@ __device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &c
   }
 }
 
+// float16 has no exponents to spare: score gradients enter their products times a power of two, chosen so that the largest
+// one possible is just below 2^15, and the accumulators are brought to a smaller power when a tile with larger ones comes.
+// Unscaled, gradients below 6e-5 lose bits (dout of 1e-4: dk off by 0.004 of its size) and those above 65504 are lost.
+template <typename T>
+constexpr bool SCALED = __is_same(T, f16_t);
+constexpr int TOP_POWER = 15, MOST_POWER = 60, LEAST_POWER = -40;  // 2^-40: the largest f16 operands at 128 elements
+// The power for values below `bound` (not a number or infinite: such a tile has no finite results).
+__device__ __forceinline__ int power_for(float bound) {
+  const int k = (int)((__float_as_uint(bound) >> 23) & 255) - 126;  // bound < 2^k
+  return max(LEAST_POWER, min(MOST_POWER, TOP_POWER - k));
+}
+__device__ __forceinline__ float pow2(int n) { return __builtin_amdgcn_ldexpf(1.0f, n); }
+// What rounding took from the output is kept times 2^11 in float16: it starts 11 bits below the output itself.
+template <typename T>
+constexpr float LO_SCALE = SCALED<T> ? 2048.0f : 1.0f;
+
 template <typename T>
 constexpr int pad() { return sizeof(T) == 2 ? 16 : 4; }
 
@@ -80,6 +96,43 @@ __device__ __forceinline__ Frag<T> zero_unless(const Frag<T> &f, bool row_ok, in
   return r;
 }
 
+// The largest magnitude among eight float16 values and `so_far`, as its bits (their order is that of the magnitudes).
+__device__ __forceinline__ unsigned top_bits(const Frag<f16_t> &f, unsigned so_far) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  union {
+    Frag<f16_t>::vec v;
+    u16x8 u;
+  } a;
+  a.v = f.v;
+  a.u &= (unsigned short)0x7fff;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) so_far = max(so_far, (unsigned)a.u[i]);
+  return so_far;
+}
+__device__ __forceinline__ float from_bits(unsigned u) {
+  union {
+    unsigned short u;
+    f16_t h;
+  } a;
+  a.u = (unsigned short)u;
+  return (float)a.h;
+}
+// Maximum over the four lanes that hold one column (l, l + 16, l + 32, l + 48), in each of them.
+__device__ __forceinline__ float col_max(float x) {
+  u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// Maximum over the wave, in every lane.
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp_mov<DPP_XOR1>(x));
+  x = fmaxf(x, dpp_mov<DPP_XOR2>(x));
+  x = fmaxf(x, dpp_mov<DPP_HALF_MIRROR>(x));
+  x = fmaxf(x, dpp_mov<DPP_MIRROR>(x));
+  return col_max(x);
+}
+
 // ROWS x DP elements on their way from memory to LDS (row stride DP + pad), THREADS threads.
 template <typename T, int ROWS, int DP, int THREADS, bool VEC>
 struct Tile {
@@ -97,13 +150,16 @@ struct Tile {
       r[k] = load8<T, VEC>(tile + row * (unsigned)stride, (i % CH) * 8, D);
     }
   }
-  __device__ __forceinline__ void store(T *lds, long row0, long rows, int D, int tid) const {
+  // top: the largest magnitude of what this thread stores (float16; as its bits)
+  template <bool TOP = false>
+  __device__ __forceinline__ void store(T *lds, long row0, long rows, int D, int tid, unsigned *top = nullptr) const {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int i = tid + k * THREADS, row = i / CH, c = (i % CH) * 8;
       if (!WHOLE && i >= ROWS * CH) break;
       const Frag<T> f = zero_unless<T, VEC>(r[k], row0 + row < rows, c, D);
       *reinterpret_cast<typename Frag<T>::vec *>(lds + row * (DP + pad<T>()) + c) = f.v;
+      if constexpr (TOP) *top = top_bits(f, *top);
     }
   }
 };
@@ -169,13 +225,7 @@ __device__ __forceinline__ void put_split(const f32x4 &x, int i0, Frag<T> &hi, F
   }
 }
 
-// Maximum / sum over the four lanes that hold one column (l, l + 16, l + 32, l + 48), in each of them.
-__device__ __forceinline__ float col_max(float x) {
-  u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
+// Their sum.
 __device__ __forceinline__ float col_sum(float x) {
   x = fold16(x, x);
   return fold32(x, x);
@@ -410,7 +460,7 @@ __global__ __launch_bounds__(256, 2) void bk_attn_kernel(AttnArgs a) {
         if (a.lo) {
           f32x4 e;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) e[r] = v[r] - (float)(T)v[r];
+          for (int r = 0; r < 4; ++r) e[r] = (v[r] - (float)(T)v[r]) * LO_SCALE<T>;
           store4<T, VEC>((T *)a.lo + (op - (T *)a.o), 16 * d + 4 * g, a.D, e);
         }
       }
@@ -446,13 +496,23 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
   const T *qp = head<T>(a.q, b, h), *gp = head<T>(a.dout, b, h), *kp = head<T>(a.k, b, hk), *vp = head<T>(a.v, b, hk);
   const float sc = a.scale * LOG2E;
   Frag<T> q[QB][NC], go[QB][NC];
-  float lse[QB], delta[QB];
+  float lse[QB], delta[QB];  // lse less the power of two that the row's score gradients carry (SCALED)
+  // SCALED: largest |v| of a tile, by wave; by row sum |do_i|, so that |do_i . v_j| <= reach max |v|, and the power.  The rows
+  // are the wave's own and its lanes' accesses stay in order.
+  __shared__ float sTop[4], sReach[SCALED<T> ? BM : 1];
+  __shared__ int sPower[SCALED<T> ? BM : 1];
+  float *reach = sReach + (SCALED<T> ? wave * WQ + m : 0);
+  int *power = sPower + (SCALED<T> ? wave * WQ + m : 0);
   f32x4 dq[ND][QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int row = w0 + 16 * i + m;
     lse[i] = INF;
     delta[i] = 0.0f;
+    if constexpr (SCALED<T>) {
+      reach[16 * i] = 0.0f;
+      power[16 * i] = MOST_POWER;
+    }
     if (q1 >= q0) {
       const long r = min(row, len - 1);
 #pragma unroll
@@ -480,13 +540,24 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
 #pragma unroll
       for (int c = 0; c < NC; ++c) mma(oo[c], go[i][c], od);
       if (a.lo) {
+        f32x4 rest = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < NC; ++c) mma(ol[c], go[i][c], od);
+        for (int c = 0; c < NC; ++c) mma(ol[c], go[i][c], rest);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) od[r] = fmaf(rest[r], 1.0f / LO_SCALE<T>, od[r]);
+      }
+      if constexpr (SCALED<T>) {
+        float l1 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) l1 += fabsf((float)go[i][c].v[e]);
+        reach[16 * i] = col_sum(l1);
       }
       const float mine = (m & 2) ? ((m & 1) ? od[3] : od[2]) : ((m & 1) ? od[1] : od[0]);
       const float dot = col_sum(g == (m >> 2) ? mine : 0.0f);  // to the four lanes that share the row
       if (row < len) {
-        lse[i] = l_;
+        lse[i] = SCALED<T> ? l_ - (float)MOST_POWER : l_;
         delta[i] = dot;
         if (g == 0) a.delta[((long)b * a.H + h) * a.L + row] = dot;
       }
@@ -504,7 +575,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
     const int j0 = kt.key0(it, BN);
     __syncthreads();
     tk.store(sK, j0, len, a.D, tid);
-    tv.store(sV, j0, len, a.D, tid);
+    if constexpr (SCALED<T>) {
+      unsigned top = 0;
+      tv.template store<true>(sV, j0, len, a.D, tid, &top);
+      const float w_ = wave_max(from_bits(top));
+      if (lane == 0) sTop[wave] = w_;
+    } else {
+      tv.store(sV, j0, len, a.D, tid);
+    }
     __syncthreads();
     if (it + 1 < kt.n) {
       const int j = kt.key0(it + 1, BN);
@@ -513,6 +591,28 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
     }
     const int view = w1 >= w0 ? tile_view(w0, w1, j0, j0 + BN - 1, a.W, a.S) : 0;
     if (!view) continue;
+    if constexpr (SCALED<T>) {
+      const float top = fmaxf(fmaxf(sTop[0], sTop[1]), fmaxf(sTop[2], sTop[3]));
+      int to[QB];
+      bool less = false;
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        to[i] = min(power[16 * i], power_for(fmaf(reach[16 * i], top, fabsf(delta[i]))));
+        less |= to[i] < power[16 * i];
+      }
+      if (__any(less)) {
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+          const float f = pow2(to[i] - power[16 * i]);
+          lse[i] += (float)(power[16 * i] - to[i]);
+          power[16 * i] = to[i];
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dq[d][i][r] *= f;
+        }
+      }
+    }
 #pragma unroll
     for (int k = 0; k < NK; k += 2) {
       Frag<T> ds[QB], dl[QB];
@@ -573,11 +673,12 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void bk_attn_dq_
     const int row = w0 + 16 * i + m;
     if (row < a.L) {
       T *op = (T *)a.dq + (((long)b * a.L + row) * a.H + h) * a.D;
+      const float back = SCALED<T> ? a.scale * pow2(-power[16 * i]) : a.scale;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = row < len && lse[i] != INF ? dq[d][i][r] * a.scale : 0.0f;
+        for (int r = 0; r < 4; ++r) v[r] = row < len && lse[i] != INF ? dq[d][i][r] * back : 0.0f;
         store4<T, VEC>(op, 16 * d + 4 * g, a.D, v);
       }
     }
@@ -599,6 +700,7 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
   __shared__ __attribute__((aligned(16))) T sQ[ROWS * LD], sG[ROWS * LD];
   __shared__ Frag<T> sF[VLDS ? 4 * 3 * NC * 64 : 1];
   __shared__ __attribute__((aligned(16))) float sL[ROWS], sD[ROWS];
+  __shared__ float sTop[4], sFar[4];  // SCALED: largest |do| and |delta| of a tile, by wave
   const int nk = SINK ? (a.S + WK - 1) / WK : (a.L + BK - 1) / BK, ns = SINK ? a.nsplit : 1;
   long w = work_item((long)a.B * a.Hk * nk * ns);
   if (w < 0) return;
@@ -628,6 +730,7 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
   Frag<T> kf[VLDS ? 1 : KB][NC], vf[VLDS ? 1 : KB][VLDS ? 1 : NC];
   Frag<T> *mine = sF + (VLDS ? wave * 3 * NC * 64 + lane : 0);  // v of both key blocks, then k of the second
   f32x4 dk[ND][KB], dv[ND][KB];
+  unsigned vtop = 0;
 #pragma unroll
   for (int i = 0; i < KB; ++i) {
 #pragma unroll
@@ -645,6 +748,7 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
       for (int c = 0; c < NC; ++c) {
         k_[c] = zero_unless<T, VEC>(k_[c], row < len, c * 32 + g * 8, a.D);
         v_[c] = zero_unless<T, VEC>(v_[c], row < len, c * 32 + g * 8, a.D);
+        if constexpr (SCALED<T>) vtop = top_bits(v_[c], vtop);
         if constexpr (VLDS) {
           mine[(i * NC + c) * 64] = v_[c];
           if (i == 0) kf[0][c] = k_[c];
@@ -656,6 +760,8 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
       }
     }
   }
+  const float vmost = SCALED<T> ? wave_max(from_bits(vtop)) * (float)a.D : 0.0f;  // |do . v| <= D max |do| max |v|
+  int power = MOST_POWER;
   const int per_head = q_to > q_from ? (int)((q_to - q_from + ROWS - 1) / ROWS) : 0, total = per_head * G;
   Tile<T, ROWS, DP, 256, VEC> tq, tg;
   float rl = INF, rd = 0.0f;
@@ -675,9 +781,20 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
     const long qi = q_from + (long)(it % per_head) * ROWS;
     __syncthreads();
     tq.store(sQ, qi, len, a.D, tid);
-    tg.store(sG, qi, len, a.D, tid);
+    if constexpr (SCALED<T>) {
+      unsigned top = 0;
+      tg.template store<true>(sG, qi, len, a.D, tid, &top);
+      const float w_ = wave_max(from_bits(top));
+      if (lane == 0) sTop[wave] = w_;
+      if (wave * 64 < ROWS) {
+        const float f_ = wave_max(tid < ROWS && qi + tid < len ? fabsf(rd) : 0.0f);
+        if (lane == 0) sFar[wave] = f_;
+      }
+    } else {
+      tg.store(sG, qi, len, a.D, tid);
+    }
     if (tid < ROWS) {
-      sL[tid] = qi + tid < len ? rl : INF;
+      sL[tid] = qi + tid < len ? (SCALED<T> ? rl - (float)TOP_POWER : rl) : INF;
       sD[tid] = qi + tid < len ? rd : 0.0f;
     }
     __syncthreads();
@@ -685,6 +802,23 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
     const int i0 = (int)qi + sub;
     const int view = i0 < len && key0 < len ? tile_view(i0, i0 + BQ - 1, key0, key0 + WK - 1, a.W, a.S) : 0;
     if (!view) continue;
+    float factor = 1.0f;  // of do . v - delta, beside the 2^15 that the probabilities carry in float16
+    if constexpr (SCALED<T>) {
+      const float top = fmaxf(fmaxf(sTop[0], sTop[1]), fmaxf(sTop[2], sTop[3]));
+      const float far = ROWS > 64 ? fmaxf(sFar[0], sFar[1]) : sFar[0];
+      const int to = min(power, __builtin_amdgcn_readfirstlane(power_for(fmaf(vmost, top, far))));
+      if (to < power) {
+        const float f = pow2(to - power);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int y = 0; y < KB; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dk[d][y][r] *= f;
+        power = to;
+      }
+      factor = pow2(power - TOP_POWER);
+    }
     Frag<T> pf[KB], pl[KB], df[KB], dl[KB];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -706,7 +840,11 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
         }
       }
       const f32x4 ls = *reinterpret_cast<const f32x4 *>(&sL[sub + 16 * x + 4 * g]);
-      const f32x4 de = *reinterpret_cast<const f32x4 *>(&sD[sub + 16 * x + 4 * g]);
+      f32x4 de = *reinterpret_cast<const f32x4 *>(&sD[sub + 16 * x + 4 * g]);
+      if constexpr (SCALED<T>) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) de[r] *= factor;
+      }
 #pragma unroll
       for (int y = 0; y < KB; ++y)
 #pragma unroll
@@ -724,7 +862,7 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           s[y][r] = exp2_fast(s[y][r]);
-          dp[y][r] = s[y][r] * (dp[y][r] - de[r]);
+          dp[y][r] = s[y][r] * (SCALED<T> ? fmaf(dp[y][r], factor, -de[r]) : dp[y][r] - de[r]);
         }
         put_split(s[y], 4 * x, pf[y], pl[y]);
         put_split(dp[y], 4 * x, df[y], dl[y]);
@@ -752,6 +890,8 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
     }
   }
   const bool parts = a.nsplit > 0;
+  const float kback = SCALED<T> ? a.scale * pow2(-power) : a.scale;
+  const float vback = SCALED<T> ? 1.0f / (1 << TOP_POWER) : 1.0f;
 #pragma unroll
   for (int y = 0; y < KB; ++y) {
     const int key = key0 + 16 * y + m;
@@ -764,8 +904,8 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (16 * d + 4 * g + r < a.D) {
-              p[16 * d + 4 * g + r] = dk[d][y][r] * a.scale;
-              p[a.D + 16 * d + 4 * g + r] = dv[d][y][r];
+              p[16 * d + 4 * g + r] = dk[d][y][r] * kback;
+              p[a.D + 16 * d + 4 * g + r] = dv[d][y][r] * vback;
             }
       }
     } else if (key < a.L) {
@@ -774,9 +914,11 @@ __global__ __launch_bounds__(256, KB == 2 && DP * (SINK ? 2 : 1) * sizeof(T) > 2
       for (int d = 0; d < ND; ++d) {
         f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = dk[d][y][r] * a.scale;
+        for (int r = 0; r < 4; ++r) v[r] = dk[d][y][r] * kback;
         store4<T, VEC>((T *)a.dk + at0, 16 * d + 4 * g, a.D, v);
-        store4<T, VEC>((T *)a.dv + at0, 16 * d + 4 * g, a.D, dv[d][y]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = dv[d][y][r] * vback;
+        store4<T, VEC>((T *)a.dv + at0, 16 * d + 4 * g, a.D, v);
       }
     }
   }

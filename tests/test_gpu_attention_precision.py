@@ -70,3 +70,41 @@ def test_single_tokens_are_as_near_as_their_rounding(B, H, Hk, D, window, sinks,
     K, V = (t.double().repeat_interleave(H // Hk, 1) for t in (k, v))
     p = torch.softmax((K @ q[:, :, -1, :, None].double())[..., 0] * D ** -0.5, -1)
     assert rounding_ratio(got, (p[..., None] * V).sum(2)) <= NEAR
+
+
+# float16 gradients over its whole range: score gradients far below its smallest steps and beyond its largest value, values so
+# small that the output is kept in whole steps of 2^-24, rows of very different size in one sequence
+ANY_SIZE = [(1024, 64, 512, 0, 1, 1, 1e-4), (1024, 64, 512, 4, 1, 1, 1e-4), (300, 64, 4, 0, 0.05, 1, 1e4), (300, 128, 4, 0, 0.02, 1, 1e4),
+            (900, 32, 8, 40, 0.02, 1, 1e4), (300, 64, 40, 3, 1, 1e-3, 1e2), (300, 64, 40, 3, 1, 1e-5, 1e4),
+            (200, 128, 30, 2, 0.1, 1e3, 1e-2), (300, 20, 60, 2, 1, 1, 1e-4)]
+
+
+@pytest.mark.parametrize("B,H,Hk,L,D,window,sinks,qk,vs,dos",
+                         [(1, 4, 1, *c) for c in ANY_SIZE] + [(6, 16, 16, *c) for c in ANY_SIZE if c[0] <= 300])
+def test_float16_gradients_of_any_size(B, H, Hk, L, D, window, sinks, qk, vs, dos):
+    q, k, v, do = (t.float() for t in inputs(B, H, Hk, L, D, F32, seed=D + L))
+    q, k, v, do = (qk * q).half(), (qk * k).half(), (vs * v).half(), (dos * do).half()
+    got = train(*(t.cuda() for t in (q, k, v, do)), window, sinks)
+    r = attention(*d64(q, k, v), window, sinks, D ** -0.5, 0.0, None, d64(do))
+    for t, n in zip(got, ("o", "dq", "dk", "dv")):
+        want = r[n]                                     # where the definition is beyond float16's largest value, so is the result
+        border = (want.abs() / 65520 - 1).abs() < 2.0 ** -11
+        over = torch.isinf(want.half())
+        assert torch.equal(torch.isinf(t.cpu())[~border], over[~border]) and not torch.isnan(t).any(), n
+        fine = ~over & ~border
+        assert rounding_ratio(t.cpu()[fine], want[fine]) <= NEAR, n
+
+
+def test_float16_gradients_of_rows_of_any_size():
+    """Each row's dout at its own power of two: dq is held row by row, dk and dv by the sizes of what reaches a key."""
+    q, k, v, do = inputs(2, 4, 2, 300, 64, F32, seed=3)
+    g = torch.Generator().manual_seed(4)
+    size = 2.0 ** torch.randint(-12, 12, (2, 4, 300, 1), generator=g)
+    q, k, v, do = q.half(), k.half(), v.half(), (size * do).half()
+    got = train(*(t.cuda() for t in (q, k, v, do)), 40, 3)
+    r = attention(*d64(q, k, v), 40, 3, 0.125, 0.0, None, d64(do))
+    for t, n in zip(got, ("o", "dq", "dk", "dv")):
+        assert rounding_ratio(t, r[n]) <= NEAR, n
+    dq, want = d64(got[1]), r["dq"]
+    off, least = (dq - want).norm(dim=-1), (want.half().double() - want).norm(dim=-1)
+    assert (off <= 2 * least + 2.0 ** -24).all()        # of a row's 64 roundings one or two fall to the other side
