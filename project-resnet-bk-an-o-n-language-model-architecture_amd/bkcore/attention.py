@@ -105,8 +105,8 @@ def sliding_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
                            positions: torch.Tensor, window: int, sinks: int = 0,
                            scale: float | None = None) -> torch.Tensor:
     """``sliding_attention`` for one token of each sequence: q (B, H, D), k and v (B, Hk, D) of the token at ``positions``
-    (B,), below 2**31, which are written into the rolling caches (see ``sliding_cache_fill``; at least ``window + sinks`` slots) in place.
-    A negative position leaves its sequence alone: output zero, cache as it was.  No gradient."""
+    (B,), which are written into the rolling caches (see ``sliding_cache_fill``; at least ``window + sinks`` slots) in place.
+    A negative position, or one from 2**31 on, leaves its sequence alone: output zero, cache as it was.  No gradient."""
     what = "sliding_attention_step"
     _heads(what, q, k, v, 3)
     window, sinks = _window(what, window, sinks)
@@ -118,7 +118,7 @@ def sliding_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_
     ops.need_shape(what, "positions", positions, (q.shape[0],))
     ops.need_device(q, positions)
     if positions.dtype == torch.int64:
-        positions = positions.to(torch.int32)
+        positions = positions.clamp(-1, 2 ** 31).to(torch.int32)      # 2**31 becomes the lowest int32: left alone too
     elif positions.dtype != torch.int32:
         raise TypeError(f"bkcore: {what}: positions are int32 or int64, not {positions.dtype}")
     with ops.on_device(q.device):

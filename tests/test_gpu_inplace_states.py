@@ -89,3 +89,15 @@ def test_inference_tensors_are_updated_too():
         caches = (torch.zeros(2, 2, 10, 16, device="cuda"), torch.zeros(2, 2, 10, 16, device="cuda"))
         attention_step(caches)
         assert (caches[0][:, :, 0] != 0).all()
+
+
+@pytest.mark.parametrize("outside", [-1, -2 ** 31, -2 ** 32, -2 ** 33 + 1, -2 ** 63, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1])
+def test_positions_outside_int32_leave_their_sequence_alone(outside):
+    """Their low 32 bits are positions that the cache has."""
+    import bkcore
+    q, k, v = rn(2, 4, 16), rn(2, 2, 16), rn(2, 2, 16)
+    kc, vc = rn(2, 2, 10, 16), rn(2, 2, 10, 16)
+    k0, v0 = kc.clone(), vc.clone()
+    o = bkcore.sliding_attention_step(q, k, v, kc, vc, torch.tensor([outside, 0], device="cuda"), 8, 2)
+    assert (o[0] == 0).all() and torch.equal(kc[0], k0[0]) and torch.equal(vc[0], v0[0])
+    assert torch.equal(o[1], v[1].repeat_interleave(2, 0)) and torch.equal(kc[1, :, 0], k[1])
