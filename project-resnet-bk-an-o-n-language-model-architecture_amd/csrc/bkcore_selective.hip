@@ -64,6 +64,10 @@ __device__ __forceinline__ float sum_states(float v) {
   return v;
 }
 
+// A state behind a chunk: a h + e.  Where d A is positive a chunk's factor may be beyond float32 although no position's is; a
+// state that is still zero stays zero then, as it does position by position.
+__device__ __forceinline__ float decayed(float a, float h, float e) { return h == 0.0f ? e : fmaf(a, h, e); }
+
 // The value of lane Q of each quad.
 // (The empty asm keeps the move a move: folded into its eight users it would make each of them a DPP instruction at 4.3
 // cycles instead of 2.4.)
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(THREADS) void bk_scan_kernel(ScanArgs a) {
       const float sd = a.aggd[at0];
       const f32x4 e = *reinterpret_cast<const f32x4 *>(a.agg + at0 * NP + sub * 4);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) h[n] = fmaf(exp2_fast(A2[n] * sd), h[n], e[n]);
+      for (int n = 0; n < 4; ++n) h[n] = decayed(exp2_fast(A2[n] * sd), h[n], e[n]);
     }
   }
   float sum_d = 0.0f;
@@ -377,7 +381,7 @@ __global__ __launch_bounds__(THREADS, 2) void bk_scan_backward_kernel(ScanArgs a
       const float sd = a.aggd[at0];
       const f32x4 e = *reinterpret_cast<const f32x4 *>(a.agg + at0 * NP + sub * 4);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) carry[n] = fmaf(exp2_fast(A2[n] * sd), carry[n], e[n]);
+      for (int n = 0; n < 4; ++n) carry[n] = decayed(exp2_fast(A2[n] * sd), carry[n], e[n]);
     }
   }
   const long ntiles = (a.L + TILE - 1) / TILE;
