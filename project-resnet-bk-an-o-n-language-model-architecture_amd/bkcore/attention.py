@@ -64,6 +64,32 @@ def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
                                                     ops.stream(q.device.index))
 
 
+def _reaches(distance: int, steps: list) -> bool:
+    """Whether `distance` is a sum of d * stride over (stride, size) with |d| < size, strides descending and each beyond the
+    reach of those behind it: two views of these strides that far apart have an element in common."""
+    if not steps:
+        return distance == 0
+    stride, size = steps[0]
+    near = distance // stride
+    return any(abs(d) < size and _reaches(distance - d * stride, steps[1:]) for d in (near, near + 1))
+
+
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors have memory in common.  Views of one memory with other strides count as sharing when one begins
+    inside the other's reach."""
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    distance = b.data_ptr() - a.data_ptr()
+    if distance >= a.numel() * a.element_size() and a.is_contiguous() or not (a.numel() and b.numel()):
+        return False
+    steps = sorted(((a.stride(i), a.shape[i]) for i in range(a.dim()) if a.shape[i] > 1), reverse=True)
+    if distance > sum(st * (n - 1) for st, n in steps) * a.element_size() + a.element_size() - 1:
+        return False
+    if a.stride() != b.stride() or a.shape != b.shape or distance % a.element_size():
+        return True
+    return _reaches(distance // a.element_size(), steps)
+
+
 def _cache(what: str, q: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int) -> int:
     """Checks the caches (B, Hk, slots, D) and returns the number of slots."""
     ops.need_device(q, k_cache, v_cache)
@@ -79,8 +105,8 @@ def _cache(what: str, q: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, v
                     raise ValueError(f"bkcore: {what}: slots of {name} overlap")
                 reach += stride * (size - 1)
         ops.need_state(what, name, c, q, tuple(c.shape), q.dtype)
-    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
-        raise ValueError(f"bkcore: {what}: k_cache and v_cache are the same memory")
+    if _share(k_cache, v_cache):
+        raise ValueError(f"bkcore: {what}: k_cache and v_cache share memory")
     if k_cache.shape[2] <= sinks:
         raise ValueError(f"bkcore: {what}: {k_cache.shape[2]} slots leave none behind {sinks} sinks")
     return k_cache.shape[2]
@@ -90,12 +116,15 @@ def sliding_cache_fill(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, 
                        lengths: torch.Tensor | None = None, sinks: int = 0) -> None:
     """Writes a prompt's keys and values (B, Hk, L, D) into rolling caches (B, Hk, slots, D): the first ``sinks`` positions
     and the last ``slots - sinks`` behind them.  Position p lives in slot p for p < sinks and in slot
-    ``sinks + (p - sinks) % (slots - sinks)`` behind; slots of no position stay as they were."""
+    ``sinks + (p - sinks) % (slots - sinks)`` behind; slots of no position stay as they were.  k and v lie outside the
+    caches."""
     what = "sliding_cache_fill"
     _heads(what, k, k, v, 4)
     _, sinks = _window(what, 1, sinks)
     ops.no_grad_through(what, k, v)
     _cache(what, k, k, k_cache, v_cache, sinks)
+    if any(_share(t, c) for t in (k, v) for c in (k_cache, v_cache)):
+        raise ValueError(f"bkcore: {what}: k or v shares memory with a cache, whose slots are written in no order")
     n = ops.lengths_arg(what, lengths, k, k.shape[0], k.shape[2])
     with ops.on_device(k.device):
         _lib.load_native().sliding_cache_fill(k, v, k_cache, v_cache, n, sinks, ops.stream(k.device.index))
