@@ -355,8 +355,8 @@ size_t bkcore_woodbury_workspace_bytes(int64_t B, int64_t N, int64_t r);
  * scan of a selective mixer, sliding-window attention with sinks.  Element types BKCORE_F32 / BF16 / F16 (`dtype`, of all
  * activations of a call); arithmetic, sums and states are float32.  Strides are in elements; the innermost dimension
  * (channels, head dimension) has stride 1.  `lengths` is NULL or B ints on the device: positions at or behind a
- * sequence's length are padding, which is never read; outputs and gradients there are zero (values outside 0..L are
- * taken as the nearest of the two).  Workspaces need 16-byte alignment.
+ * sequence's length are padding, whose values do not matter (kernels may load and drop them); outputs and gradients
+ * there are zero (lengths outside 0..L are taken as the nearest of the two).  Workspaces need 16-byte alignment.
  */
 
 /* Layer norm over D elements, rows of stride ldx: y = (x - mean) / sqrt(var + eps) * weight + bias, y contiguous.

@@ -3,7 +3,7 @@ hybrid layer without its block borders (reference src/models/phase7/hybrid_atten
 and, on a rolling key / value cache, for single tokens.
 
 Query i of a sequence sees the keys j <= i with ``i - j < window`` or ``j < sinks``.  Positions at or behind ``lengths``
-(B,) are padding of a right-padded batch: they are never read, outputs and gradients there are zero."""
+(B,) are padding of a right-padded batch: their values do not matter, outputs and gradients there are zero."""
 from __future__ import annotations
 
 import torch
@@ -51,8 +51,8 @@ def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
     strides (slices of one projection).  The result (B, H, L, D) has its heads inside a position in memory.
 
     Scores, softmax and sums are float32; probabilities and score gradients enter their products as two values of the
-    operands' type, so results are as near as their own rounding.  A non-finite key
-    or value inside a sequence may reach any row that works on the same tile of keys, not only those that see it."""
+    operands' type, so results are as near as their own rounding.  A non-finite key or value inside a sequence may reach
+    any row that works on the same tile of keys, not only those that see it."""
     what = "sliding_attention"
     _heads(what, q, k, v, 4)
     B, H, T, D = q.shape

@@ -2,8 +2,8 @@
 training and for single tokens.  They stand beside ``fused_associative_scan``, the plain accumulation of the reference's
 global path (src/models/phase1/ar_ssm_layer.py:517-525): here the decay and what enters the state depend on the input.
 
-Channels are innermost: (B, L, C).  Positions at or behind ``lengths`` (B,) are padding of a right-padded batch: they are
-never read, outputs and gradients there are zero, and a returned state is the one behind the last position inside."""
+Channels are innermost: (B, L, C).  Positions at or behind ``lengths`` (B,) are padding of a right-padded batch: their
+values do not matter, outputs and gradients there are zero, and a returned state is the one behind the last position inside."""
 from __future__ import annotations
 
 import torch

@@ -11,13 +11,14 @@
 // plus two exchanges.  The other operand of that product (V, or K, Q, dO in the backward) is contracted over its rows: it
 // is read from LDS through the transposing read (16-bit) or element by element (float32).
 //
-// What bounds it: in the prompts and in training the vector unit (one exponential and about ten instructions a score), the
-// matrix unit and LDS take a like share each of a tile's time, and two waves a SIMD hide only part of one behind another.
-// Measured at 2 x 16 heads x 8192 x 128 bf16 over 4 key heads, window 1024, 4 sinks: forward 246 us (129 GFLOP: 0.53 PFLOP/s),
-// dq with delta 345 (delta in a launch of its own: 325 + 31), dk and dv 424 + 44 + 5 (the sinks' part and its join apart);
-// both form the scores again, so the backward does nine products of this size for the five it needs (two of the nine are
-// the second halves of the score gradients); 4 x 8 heads x 3001 ragged x 64 f16, window 500: 31.  The single-token step is
-// bound by the cache's bytes: 64 sequences x 32 heads over 8 x 4100 slots x 128 bf16 in 171 + 5 us = 5.7 TB/s.
+// What bounds it: in the prompts and in training the vector unit (17 instructions a visible score in the forward), the
+// matrix unit and LDS, of which two waves a SIMD hide only part behind one another.
+// Measured at 2 x 16 heads x 8192 x 128 bf16 over 4 key heads, window 1024, 4 sinks (share of the time that the vector unit,
+// the matrix unit and LDS are busy): forward 288 us (56, 33, 17 %), dq with delta 332 (44, 39, 20 %), dk and dv 465 (37, 38,
+// 27 %) + 44 + 5 (the sinks' part and its join).  Products of 65 GFLOP: the forward does three for two (the second half of
+// the probabilities), the backward ten for five (both its kernels form the scores again, and three are second halves).
+// 4 x 8 heads x 3001 ragged x 64 f16, window 500: 37.  The single-token step is bound by the cache's bytes: 64 sequences x
+// 32 heads over 8 x 4100 slots x 128 bf16 in 171 + 5 us = 5.7 TB/s.
 #include "bkcore_attention.h"
 
 namespace bk {

@@ -2,9 +2,9 @@
 // for single tokens.
 //   pre_t = bias + sum_k w_k x_{t-K+1+k},  y_t = pre_t or silu(pre_t);  x at t < 0 is the carried state, or zero
 //   g_t = dy_t act'(pre_t);  dx_t = sum_k w_k g_{t+K-1-k};  dw_k = sum g_t x_{t-K+1+k};  db = sum g_t
-// Positions at or behind a sequence's length are padding: they are never read, y and dx there are zero.
+// Positions at or behind a sequence's length are padding: what is loaded there is dropped, y and dx there are zero.
 // HBM-bound: 2 e bytes an element forward, 3 e backward (8 x 2048 x 1024 bf16: 18.5 us = 3.6 TB/s, and 31.9 + 4 us =
-// 2.8 TB/s).  A thread holds V neighbouring channels (16 bytes a position forward, 4 channels backward, where five sums and
+// 2.8 TB/s; the forward's vector unit is busy 32 % of the time, the backward's 66 %).  A thread holds V neighbouring channels (16 bytes a position forward, 4 channels backward, where five sums and
 // two windows a channel take the registers) and walks a stretch of positions with the last K - 1 inputs in registers; only
 // the K - 1 positions in front of its stretch are read twice, from cache.  Arithmetic and sums are float32.
 #include "bkcore_types.h"
@@ -210,66 +210,66 @@ __global__ __launch_bounds__(BWD_CH *BWD_SEGS) void bk_conv_backward_kernel(Conv
 #pragma unroll
       for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
     for (long tb0 = t0; tb0 < t1 + K - 1; tb0 += UNDER) {
-    cur = next;
-    if (tb0 + UNDER < t1 + K - 1) fetch(tb0 + UNDER);
+      cur = next;
+      if (tb0 + UNDER < t1 + K - 1) fetch(tb0 + UNDER);
 #pragma unroll
-    for (int j = 0; j < UNDER; ++j) {
-      const long t = tb0 + j;
-      if (t >= t1 + K - 1) break;
-      if (t < len) {
-        float d[V];
-        cur.x[j].get(true, h[K - 1]);
-        cur.g[j].get(true, d);
+      for (int j = 0; j < UNDER; ++j) {
+        const long t = tb0 + j;
+        if (t >= t1 + K - 1) break;
+        if (t < len) {
+          float d[V];
+          cur.x[j].get(true, h[K - 1]);
+          cur.g[j].get(true, d);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (a.silu) {
-            float s = bias[i];
+          for (int i = 0; i < V; ++i) {
+            if (a.silu) {
+              float s = bias[i];
 #pragma unroll
-            for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
-            const float sg1 = sigmoid(s);
-            d[i] *= sg1 * fmaf(s, 1.0f - sg1, 1.0f);
+              for (int k = 0; k < K; ++k) s = fmaf(w[k][i], h[k][i], s);
+              const float sg1 = sigmoid(s);
+              d[i] *= sg1 * fmaf(s, 1.0f - sg1, 1.0f);
+            }
+            g[K - 1][i] = d[i];
+            if (t < t1) {
+              db[i] += d[i];
+#pragma unroll
+              for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d[i], h[k][i], dw[k][i]);
+            }
           }
-          g[K - 1][i] = d[i];
-          if (t < t1) {
-            db[i] += d[i];
+        } else {
 #pragma unroll
-            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d[i], h[k][i], dw[k][i]);
+          for (int i = 0; i < V; ++i) h[K - 1][i] = g[K - 1][i] = 0.0f;
+        }
+        const long p = t - (K - 1);  // the position that is complete now
+        if (p >= t0 || (t0 == 0 && a.dinit)) {
+          float o[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) s = fmaf(w[k][i], g[K - 1 - k][i], s);
+            o[i] = s;
           }
-        }
-      } else {
+          const long j = p - ((long)len - (K - 1));  // its place in the final state
+          if (a.dfinal && j >= 0 && p < len) {
+            float f[V];
+            load_piece<T, V, AL>((const T *)a.dfinal + ((long)b * (K - 1) + j) * a.C + c, f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[K - 1][i] = g[K - 1][i] = 0.0f;
+            for (int i = 0; i < V; ++i) o[i] += f[i];
+          }
+          if (p >= t0)
+            Piece<T, V, AL>::store(dx + p * a.C, o);
+          else
+            Piece<T, V, AL>::store((T *)a.dinit + ((long)b * (K - 1) + (p + K - 1)) * a.C + c, o);
+        }
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            h[k][i] = h[k + 1][i];
+            g[k][i] = g[k + 1][i];
+          }
       }
-      const long p = t - (K - 1);  // the position that is complete now
-      if (p >= t0 || (t0 == 0 && a.dinit)) {
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float s = 0.0f;
-#pragma unroll
-          for (int k = 0; k < K; ++k) s = fmaf(w[k][i], g[K - 1 - k][i], s);
-          o[i] = s;
-        }
-        const long j = p - ((long)len - (K - 1));  // its place in the final state
-        if (a.dfinal && j >= 0 && p < len) {
-          float f[V];
-          load_piece<T, V, AL>((const T *)a.dfinal + ((long)b * (K - 1) + j) * a.C + c, f);
-#pragma unroll
-          for (int i = 0; i < V; ++i) o[i] += f[i];
-        }
-        if (p >= t0)
-          Piece<T, V, AL>::store(dx + p * a.C, o);
-        else
-          Piece<T, V, AL>::store((T *)a.dinit + ((long)b * (K - 1) + (p + K - 1)) * a.C + c, o);
-      }
-#pragma unroll
-      for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          h[k][i] = h[k + 1][i];
-          g[k][i] = g[k + 1][i];
-        }
-    }
     }
   }
   if (!a.part) return;

@@ -23,10 +23,10 @@
 // across workgroups by a second launch; every order is fixed, results do not change from run to run.
 // States, statistics and sums are float32 whatever the operands' type.
 //
-// Measured at 4 x 2048 positions x 1024 channels x 16 states, bf16: chunks' ends 34 us, forward 52, adjoint's ends 38,
-// backward 158 (512 x 16 positions a SIMD: 28, 42, 31 and 122 vector instructions a position, busy 75 % of the time; the
-// rest is the start of a chunk and the barriers), both sums 10.  8191 positions x 512 channels f32: 20 + 35.  256 tokens x
-// 2048 channels: 16.8 us (4.2 TB/s).
+// Measured at 4 x 2048 positions x 1024 channels x 16 states, bf16: chunks' ends 34 us, forward 53, adjoint's ends 38,
+// backward 160 (four waves a SIMD of 128 positions each: 28, 43, 31 and 123 vector instructions a position; the vector unit
+// is busy 65, 76, 69 and 77 % of the time), both sums 10.  8191 positions x 512 channels f32: 20 + 37.  256 tokens x 2048
+// channels: 17 us (4.2 TB/s).
 #include "bkcore_types.h"
 
 namespace {
@@ -640,8 +640,8 @@ __global__ __launch_bounds__(256) void bk_scan_step_kernel(ScanArgs a, float *__
 inline int lanes_per_channel(int64_t N) { return N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 // Chunks of the time axis: one while the channels alone give every SIMD a wave (cutting adds a pass over the inputs),
-// else enough for four waves a SIMD, of at least four tiles each (4 x 2048 positions x 1024 channels, both launches of the
-// forward: 97 us at two waves, 86 at four, 95 at six).
+// else enough for four waves a SIMD, of at least four tiles each (4 x 2048 positions x 1024 channels, 256 waves uncut, both
+// launches of the forward: 97 us at two waves a SIMD, 86 at four, 95 at six; other numbers of channels are not measured).
 struct Plan {
   int lpc, nct, S, chunk;
 };

@@ -113,8 +113,8 @@ __device__ __forceinline__ float wave_sum(float x) {
   return fold32(x, x);
 }
 
-// exp(x) through the base-2 instruction: about one part in 2^22 at |x| <= 16, growing with |x| by the rounding of the
-// product x log2(e).
+// exp(x) through the base-2 instruction: one part in 2^21 at |x| <= 4, 2^20 at |x| <= 16, growing with |x| by the rounding
+// of the product x log2(e).
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float sigmoid(float x) {
