@@ -52,7 +52,7 @@ def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
 
     Scores, softmax and sums are float32; probabilities and score gradients enter their products as two values of the
     operands' type, so results are as near as their own rounding.  A non-finite key or value inside a sequence may reach
-    any row that works on the same tile of keys, not only those that see it."""
+    any row that works on the same tile of keys, not only those that see it, and leave NaN where the formula is infinite."""
     what = "sliding_attention"
     _heads(what, q, k, v, 4)
     B, H, T, D = q.shape
@@ -64,30 +64,32 @@ def sliding_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window:
                                                     ops.stream(q.device.index))
 
 
-def _reaches(distance: int, steps: list) -> bool:
-    """Whether `distance` is a sum of d * stride over (stride, size) with |d| < size, strides descending and each beyond the
-    reach of those behind it: two views of these strides that far apart have an element in common."""
-    if not steps:
-        return distance == 0
-    stride, size = steps[0]
-    near = distance // stride
-    return any(abs(d) < size and _reaches(distance - d * stride, steps[1:]) for d in (near, near + 1))
+def _meet(distance: int, a: list, b: list) -> bool:
+    """Whether an element of b, which begins `distance` behind a, is one of a's; (stride, size) of either's dimensions with
+    strides descending.  Dimensions of equal stride are told apart exactly; where the largest strides left differ, views whose
+    reaches meet count as meeting."""
+    if not -sum(s * (n - 1) for s, n in b) <= distance <= sum(s * (n - 1) for s, n in a):
+        return False
+    if not a or not b or a[0][0] != b[0][0] or a[0][0] == 0:
+        return True
+    (stride, na), (_, nb) = a[0], b[0]
+    a, b = a[1:], b[1:]
+    least = -(-(-sum(s * (n - 1) for s, n in b) - distance) // stride)
+    most = (sum(s * (n - 1) for s, n in a) - distance) // stride
+    return any(_meet(distance + d * stride, a, b) for d in range(max(least, 1 - na), min(most, nb - 1) + 1))
 
 
 def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors have memory in common.  Views of one memory with other strides count as sharing when one begins
-    inside the other's reach."""
+    """Whether two tensors of one type have memory in common."""
     if a.data_ptr() > b.data_ptr():
         a, b = b, a
-    distance = b.data_ptr() - a.data_ptr()
-    if distance >= a.numel() * a.element_size() and a.is_contiguous() or not (a.numel() and b.numel()):
+    size, distance = a.element_size(), b.data_ptr() - a.data_ptr()
+    if distance >= a.numel() * size and a.is_contiguous() or not (a.numel() and b.numel()):
         return False
-    steps = sorted(((a.stride(i), a.shape[i]) for i in range(a.dim()) if a.shape[i] > 1), reverse=True)
-    if distance > sum(st * (n - 1) for st, n in steps) * a.element_size() + a.element_size() - 1:
-        return False
-    if a.stride() != b.stride() or a.shape != b.shape or distance % a.element_size():
-        return True
-    return _reaches(distance // a.element_size(), steps)
+    steps = [sorted(((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1), reverse=True) for t in (a, b)]
+    if distance % size:      # elements that straddle one another: by their reach
+        return distance < (sum(s * (n - 1) for s, n in steps[0]) + 1) * size
+    return _meet(distance // size, *steps)
 
 
 def _cache(what: str, q: torch.Tensor, k: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int) -> int:

@@ -44,6 +44,29 @@ def test_sharing_of_other_views():
     assert not _share(k, v)
 
 
+def test_sharing_is_never_missed_between_views_of_any_strides():
+    base = torch.zeros(3000)
+    g = torch.Generator().manual_seed(0)
+    r = lambda lo, hi: int(torch.randint(lo, hi, (), generator=g))
+    seen = set()
+    for _ in range(3000):
+        a, b = (torch.as_strided(base, [r(1, 4) for _ in range(4)], [(0, 1, 2, 3, 5, 12, 60, 200)[r(0, 8)] for _ in range(4)], r(0, 300))
+                for _ in range(2))
+        share = bool(cells(a) & cells(b))
+        seen.add(share)
+        assert _share(a, b) or not share
+        assert _share(a, b) == _share(b, a)
+    assert seen == {True, False}
+
+
+def test_prompts_and_caches_in_one_slab_a_sequence_do_not_share():
+    slab = torch.zeros(3, 1000)                                   # prompt, keys, values of a sequence one behind the other
+    k = slab[:, :160].view(3, 5, 2, 16).transpose(1, 2)
+    kc, vc = (slab[:, at:at + 320].view(3, 2, 10, 16) for at in (160, 480))
+    assert not _share(k, kc) and not _share(k, vc) and not _share(kc, vc)
+    assert _share(k, slab[:, 159:479].view(3, 2, 10, 16)) and _share(vc, slab[:, 479:799].view(3, 2, 10, 16))
+
+
 @pytest.mark.gpu
 def test_caches_that_share_a_part_are_refused():
     if not torch.cuda.is_available():
